@@ -1,7 +1,7 @@
 """Build libvitk.so (the C-ABI HIP library) in-tree with hipcc for gfx950.
 
 Called by ``__graft_entry__.build()`` and by ``python -m vit_amd._build``.  Objects are
-rebuilt only when their source (or common.h) is newer; the .so lives in ``vit_amd/lib`` so
+rebuilt only when their source, a header or this file (the flags) is newer; the .so lives in ``vit_amd/lib`` so
 it travels with the tree to the GPU box (it is git-ignored, not gpurun-ignored).
 """
 import os
@@ -14,8 +14,12 @@ CSRC = os.path.join(HERE, 'csrc')
 LIBDIR = os.path.join(HERE, 'lib')
 OBJDIR = os.path.join(LIBDIR, 'obj')
 LIB = os.path.join(LIBDIR, 'libvitk.so')
-SOURCES = ['runtime.hip', 'gemm.hip', 'gemm256.hip', 'norm_act.hip', 'attention.hip', 'attention_bwd.hip', 'attention_band.hip', 'attention_lai.hip', 'favor.hip', 'favor_fast.hip', 'optim.hip', 'loss.hip']
-FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=fast', '-Wno-unused-result']
+SOURCES = ['runtime.hip', 'gemm.hip', 'gemm256.hip', 'norm_act.hip', 'attention.hip', 'attention_bwd.hip', 'attention_band.hip', 'attention_lai.hip', 'favor.hip', 'favor_fast.hip', 'optim.hip', 'loss.hip', 'rotary.hip', 'window.hip',
+           'window_decode.hip']
+# packed-fp32-ops off: some forms of the packed fp32 instructions that hipcc makes of ordinary float code have given wrong
+# results on this hardware now and then
+FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=fast', '-Wno-unused-result',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _hipcc():
@@ -29,7 +33,8 @@ def build(verbose=True, force=False):
     os.makedirs(OBJDIR, exist_ok=True)
     hipcc = _hipcc()
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
-    hdr_mtime = max(os.path.getmtime(os.path.join(CSRC, f)) for f in os.listdir(CSRC) if f.endswith('.h'))
+    hdr_mtime = max([os.path.getmtime(os.path.join(CSRC, f)) for f in os.listdir(CSRC) if f.endswith('.h')]
+                    + [os.path.getmtime(os.path.abspath(__file__))])
     jobs = []
     objs = []
     for s in srcs:
