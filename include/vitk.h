@@ -267,6 +267,62 @@ int vitk_ce_smooth_fwd_static(int B, int C, const float* logits, long ld, const 
                               float* lse, float* loss, void* stream);
 int vitk_ce_static_max_rows(void);
 
+/* ---- long token sequences: rotary positions, query / key norms, sliding-window attention with sinks, its ring cache.
+ * No counterpart in the reference.  Here a tensor [B][N][H][dh] is (pointer, sb, sn, sh): element (b, n, h, d) at
+ * b*sb + n*sn + h*sh + d (a slice of a packed projection); outputs without strides are contiguous [B][N][H][dh].
+ *
+ * Rotary table: table[p][i] = mul * (cos, sin)(positions[p][i / per] * freqs[i % per]), per = pairs / axes, fp32
+ * [rows][pairs][2]; the angles and their sines are computed in fp64.  positions [rows][axes]: pos_kind 0 int32, 1 int64,
+ * 2 fp32, 3 fp64.  freqs: HOST memory, `per` (<= 128) doubles, read during the call. */
+int vitk_rotary_table(int pos_kind, int axes, long rows, const void* positions, int pairs, const double* freqs,
+                      double mul, float* table, void* stream);
+/* y = x with its first `rot` elements of every head turned: pair i is (i, i + rot/2), or (2i, 2i+1) when interleaved;
+ * (a, b) -> (a c - b s, b c + a s) with (c, s) of pair i in the token's table row; the rest is copied.  inverse: s -> -s
+ * (the adjoint, i.e. the backward).  Token (b, n) takes row pos[b*N + n] (pos64: int64 ids, else int32), or offset + n with
+ * pos NULL; a row outside the table makes the token's rotated elements NaN.  table: 16-byte aligned. */
+int vitk_rotary(int dtype, int inverse, int interleaved, int B, int N, int H, int dh, const void* x, long sb, long sn, long sh,
+                const float* table, long table_rows, int rot, const void* pos, int pos64, long offset, void* y, void* stream);
+/* RMS norm of every head of queries and keys, then vitk_rotary's turn, in one pass: y = R(gamma x / sqrt(mean x^2 + eps)).
+ * gamma_q / gamma_k: fp32 [dh] or NULL (ones).  rot = 0: no rotation (table may be NULL).  dh <= 128.  Backward: dx (contiguous)
+ * from x and dy; dgamma_q / dgamma_k (fp32 [dh], may be NULL) are OVERWRITTEN with the sums over all rows, in a fixed order;
+ * they need a workspace of vitk_qk_norm_rotary_bwd_workspace_bytes(dh). */
+int vitk_qk_norm_rotary_fwd(int dtype, int interleaved, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn,
+                            long qh, const void* k, long kb, long kn, long kh, const float* gamma_q, const float* gamma_k,
+                            float eps, const float* table, long table_rows, int rot, const void* pos, int pos64, long offset,
+                            void* yq, void* yk, void* stream);
+long vitk_qk_norm_rotary_bwd_workspace_bytes(int dh);
+int vitk_qk_norm_rotary_bwd(int dtype, int interleaved, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn,
+                            long qh, const void* k, long kb, long kn, long kh, const float* gamma_q, const float* gamma_k,
+                            float eps, const float* table, long table_rows, int rot, const void* pos, int pos64, long offset,
+                            const void* dyq, long gqb, long gqn, long gqh, const void* dyk, long gkb, long gkn, long gkh,
+                            void* dxq, void* dxk, float* dgamma_q, float* dgamma_k, void* workspace, void* stream);
+/* Attention of query i over the keys j with |i - j| <= window, and the first `sinks` keys always (causal: only j <= i);
+ * window < 0: every key.  Query head h reads key head h / (Hq / Hk).  lengths (int32 [B], may be NULL): tokens of each padded
+ * sequence; rows past it are not read, their outputs and gradients are 0.  dh: a multiple of 8 up to 128; pointers and strides
+ * 16-byte aligned.  lse [B][Hq][N] fp32 (may be NULL in a forward without backward): log2 of the softmax sum, +inf for a row that
+ * sees nothing (its output is 0).  The backward sums nothing with atomics. */
+int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
+                         const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
+                         int window, int sinks, int causal, const int* lengths, void* out, float* lse, void* stream);
+long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, int Hq, int Hk, int dh, int window, int sinks);
+int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
+                         const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
+                         int window, int sinks, int causal, const int* lengths, const void* out, const float* lse,
+                         const void* dout, long ob, long on, long oh, void* dq, void* dk, void* dv, void* workspace, void* stream);
+/* One new token a sequence: its k / v [B][Hk][dh] go into the ring cache [B][Hk][C][dh] (token p in slot p for p < sinks, else
+ * sinks + (p - sinks) % (C - sinks)) and its q [B][Hq][dh] attends (causal, as above) to what is visible there.  lengths
+ * (int32 [B], device): tokens before the new one, not advanced here; < 0: the sequence is skipped (out 0, cache untouched).
+ * C >= sinks + window + 1; with window < 0 slot p is token p, and a sequence with lengths[b] >= C gets NaN and writes nothing. */
+long vitk_window_decode_workspace_bytes(int dtype, int B, int Hq, int Hk, int dh, int C, int window, int sinks);
+int vitk_window_decode(int dtype, int B, int Hq, int Hk, int dh, const void* q, long qb, long qh, const void* k, long kb,
+                       long kh, const void* v, long vb, long vh, void* k_cache, void* v_cache, int C, const int* lengths,
+                       float scale, int window, int sinks, void* out, void* workspace, void* stream);
+/* Prompts of N (or lengths[b]) tokens into empty ring caches: every slot takes the last token that belongs in it, slots that
+ * the prompt does not reach are left as they are. */
+int vitk_window_cache_fill(int dtype, int B, int N, int Hk, int dh, const void* k, long kb, long kn, long kh, const void* v,
+                           long vb, long vn, long vh, const int* lengths, void* k_cache, void* v_cache, int C, int sinks,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

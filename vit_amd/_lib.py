@@ -77,6 +77,24 @@ _SIGNATURES = {
     'vitk_favor_pos_attn_bwd': ([c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_long, c_vp,
                                  c_float, c_float, c_vp, c_vp, c_vp, c_vp, c_long, c_vp, c_vp, c_vp, c_long, c_vp,
                                  c_vp, c_vp, c_vp], c_int),
+    'vitk_rotary_table': ([c_int, c_int, c_long, c_vp, c_int, c_vp, c_double, c_vp, c_vp], c_int),
+    'vitk_rotary': ([c_int] * 7 + [c_vp, c_long, c_long, c_long, c_vp, c_long, c_int, c_vp, c_int, c_long, c_vp, c_vp], c_int),
+    'vitk_qk_norm_rotary_fwd': ([c_int] * 7 + [c_vp, c_long, c_long, c_long] * 2
+                                + [c_vp, c_vp, c_float, c_vp, c_long, c_int, c_vp, c_int, c_long, c_vp, c_vp, c_vp], c_int),
+    'vitk_qk_norm_rotary_bwd_workspace_bytes': ([c_int], c_long),
+    'vitk_qk_norm_rotary_bwd': ([c_int] * 7 + [c_vp, c_long, c_long, c_long] * 2
+                                + [c_vp, c_vp, c_float, c_vp, c_long, c_int, c_vp, c_int, c_long]
+                                + [c_vp, c_long, c_long, c_long] * 2 + [c_vp] * 6, c_int),
+    'vitk_window_attn_fwd': ([c_int] * 6 + [c_vp, c_long, c_long, c_long] * 3
+                             + [c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp], c_int),
+    'vitk_window_attn_bwd_workspace_bytes': ([c_int] * 8, c_long),
+    'vitk_window_attn_bwd': ([c_int] * 6 + [c_vp, c_long, c_long, c_long] * 3
+                             + [c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_long, c_long, c_long]
+                             + [c_vp] * 5, c_int),
+    'vitk_window_decode_workspace_bytes': ([c_int] * 8, c_long),
+    'vitk_window_decode': ([c_int] * 5 + [c_vp, c_long, c_long] * 3
+                           + [c_vp, c_vp, c_int, c_vp, c_float, c_int, c_int, c_vp, c_vp, c_vp], c_int),
+    'vitk_window_cache_fill': ([c_int] * 5 + [c_vp, c_long, c_long, c_long] * 2 + [c_vp, c_vp, c_vp, c_int, c_int, c_vp], c_int),
 }
 
 

@@ -1,0 +1,828 @@
+// Attention with a sliding window and sinks over long token sequences: forward and backward.
+//
+//   visible(i, j) = (|i - j| <= w  or  j < S  or  w < 0)  and  (not causal or j <= i)  and  i, j < length of the sequence
+//   P_ij = exp(scale q_i . k_j - lse_i),  o_i = sum_j P_ij v_j        over the visible j; a row that sees nothing is zero
+//   D_i = do_i . o_i,  dS_ij = P_ij (do_i . v_j - D_i)
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij do_i   (dk, dv: over the group's heads)
+//
+// Only tiles that hold a visible pair are touched: a block of queries walks its window's key tiles and the sinks' tiles
+// before (or after) them.  Scores are made transposed, S^T[key][query] = K Q^T by 32 x 32 x 16 MFMA, so a lane owns one
+// query: the running maximum and sum are one value a lane, and the probability tile is already the B operand of
+// O^T += V^T P^T (the order of the contraction's 16 keys is the accumulator's own; V^T fragments come from the row-major
+// V tile in LDS by transpose reads in that same order).  Nothing of size N x N exists and nothing is summed by atomics:
+// the backward makes the scores twice (queries' kernel, keys' kernel).  Sums, maxima and the softmax are fp32; with bf16
+// inputs P and dS are rounded to bf16 as operands of their MFMA, each once.
+#include "common.h"
+
+namespace vitk {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+// D(32x32) += A(32x16) B(16x32).  Frag convention here: lane l holds row (A) / column (B) l & 31, k = 8 (l >> 5) + e.
+// D: register r of lane l is row 8 (r >> 2) + 4 (l >> 5) + (r & 3), column l & 31.  The fp32 form feeds element e of both
+// halves to step e: the same permutation of k on both sides.
+__device__ __forceinline__ f32x16 mma32(const Frag<__bf16>& a, const Frag<__bf16>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma32(const Frag<float>& a, const Frag<float>& b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+    return c;
+}
+// accumulator rows 16 s .. 16 s + 15 as a B fragment: element e is row 16 s + 8 (e >> 2) + 4 (l >> 5) + (e & 3)
+template <typename T> __device__ __forceinline__ void acc_frag(Frag<T>& f, const f32x16& a, int s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) frag_set_f(f, e, a[8 * s + e]);
+}
+// the A fragment that goes with it: columns col0 + (l & 31) of a row-major LDS image, rows row0 + the order above.
+// bf16: transpose reads -- lane 4 q + p of 16 supplies row q, columns 4 p .. 4 p + 3, and receives column l & 15 of the 4
+// rows; needs every lane of the wave.
+__device__ __forceinline__ void col_frag32(Frag<__bf16>& f, const __bf16* img, int ld, int row0, int col0, int lane) {
+    const int i = lane & 15, q = i >> 2, p = i & 3;
+    const __bf16* a = img + (row0 + 4 * (lane >> 5) + q) * ld + col0 + 16 * ((lane >> 4) & 1) + 4 * p;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)a);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(a + 8 * ld));
+    const s16x8 r = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    f.v = __builtin_bit_cast(bf16x8, r);
+}
+__device__ __forceinline__ void col_frag32(Frag<float>& f, const float* img, int ld, int row0, int col0, int lane) {
+    const float* a = img + (row0 + 4 * (lane >> 5)) * ld + col0 + (lane & 31);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = a[(8 * (e >> 2) + (e & 3)) * ld];
+}
+template <typename T, int LD> __device__ __forceinline__ void row_frag32(Frag<T>& f, const T* img, int row0, int kk, int lane) {
+    frag_load(f, img + (row0 + (lane & 31)) * LD + 16 * kk + 8 * (lane >> 5));
+}
+
+struct View {                     // element (b, n, h, d) at b*sb + n*sn + h*sh + d
+    const void* p;
+    long sb, sn, sh;
+};
+struct WindowParams {
+    View q, k, v, dout;           // dout: backward
+    const void* o;                // backward: the forward's output, [B][N][Hq][dh]
+    void *out, *dk, *dv;          // out: o in the forward, dq in the queries' backward kernel; all [B][N][H][dh]
+    float* lse;                   // [B][Hq][N]: log2 of the softmax sum, maximum included; +inf where a row sees nothing
+    float* delta;                 // [B][Hq][N]: D_i, written by the queries' kernel for the keys' kernel
+    float* part;                  // sinks' partial sums [B*Hk][key tiles][chunks][dk, dv][DP][32] fp32
+    const int* lengths;           // [B] or NULL
+    int B, N, Hq, Hk, G, dh;
+    int w, S, causal;
+    int tiles;                    // query tiles / key tiles of a sequence
+    int key0;                     // keys' kernel: first key (the sinks before it have their own launch)
+    int chunks, per_chunk;        // sinks' launch: query tiles are dealt to `chunks` workgroups
+    long total;                   // workgroups that have work (the grid is rounded up to whole rounds of the 8 XCDs)
+    float scale, sc2;             // sc2 = scale * log2(e)
+};
+
+// Workgroups are dealt to the 8 XCDs in turn; neighbours in the work (same keys, other head of the group; next query tile)
+// should share an L2, so XCD x takes the x-th eighth of the work in order.
+__device__ __forceinline__ long xcd_order(long total) {
+    const long per = (total + 7) / 8;
+    const long id = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    return (blockIdx.x >> 3) < per && id < total ? id : -1;
+}
+
+template <typename T, int DP> struct WCfg {
+    static constexpr int EPC = 16 / sizeof(T);          // elements of a 16-byte chunk
+    static constexpr int CPR = DP / EPC;                // chunks of a staged row
+    static constexpr int LD = DP + EPC;                 // LDS row stride: 16 bytes of padding spread the rows over the banks
+};
+
+// Rows [row0, row0 + ROWS) of a strided matrix through registers into LDS; rows outside [0, hi) and columns >= dh are zero.
+template <typename T, int DP, int ROWS, int NT> struct Stager {
+    using C = WCfg<T, DP>;
+    static constexpr int CH = ROWS * C::CPR / NT;
+    static_assert(CH * NT == ROWS * C::CPR, "a tile is a whole number of chunks a thread");
+    u32x4 r[CH];
+    __device__ __forceinline__ void load(const T* g, long sn, int row0, int hi, int dh) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int idx = threadIdx.x + c * NT;
+            const int row = row0 + idx / C::CPR, d = (idx % C::CPR) * C::EPC;
+            r[c] = u32x4{0, 0, 0, 0};
+            if (row < hi && d < dh) r[c] = *reinterpret_cast<const u32x4*>(g + (long)row * sn + d);
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int idx = threadIdx.x + c * NT;
+            *reinterpret_cast<u32x4*>(lds + (idx / C::CPR) * C::LD + (idx % C::CPR) * C::EPC) = r[c];
+        }
+    }
+};
+
+// this wave's 32 rows of a strided matrix as fragments (rows outside [0, hi) are zero)
+template <typename T, int DP>
+__device__ __forceinline__ void own_rows(Frag<T> (&f)[DP / 16], const T* g, long sn, int row, int hi, int dh, int lane) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        const int d = 16 * kk + 8 * (lane >> 5);
+        if (row < hi && d < dh) frag_load(f[kk], g + (long)row * sn + d);
+        else frag_zero(f[kk]);
+    }
+}
+
+// X^T[d][row] (a lane owns a row) times `mul` -> rows [row0, row0 + 32) of [.][dh] with row stride ldg, turned in LDS so
+// that the stores are whole chunks; rows >= hi are not written.  Only this wave's part of LDS is used.
+template <typename T, int DP>
+__device__ __forceinline__ void put_rows(const f32x16 (&x)[DP / 32], float mul, bool zero, T* lds, T* g, long ldg, int row0, int hi, int dh,
+                                         int lane) {
+    using C = WCfg<T, DP>;
+    typedef __attribute__((ext_vector_type(4))) T T4;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            T4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (T)(zero ? 0.f : x[t][4 * q + e] * mul);
+            *reinterpret_cast<T4*>(lds + (lane & 31) * C::LD + 32 * t + 8 * q + 4 * (lane >> 5)) = v;
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int idx = lane; idx < 32 * C::CPR; idx += 64) {
+        const int r = idx / C::CPR, d = (idx % C::CPR) * C::EPC;
+        if (row0 + r < hi && d < dh)
+            *reinterpret_cast<u32x4*>(g + (long)(row0 + r) * ldg + d) = *reinterpret_cast<const u32x4*>(lds + r * C::LD + d);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// The key tiles of BK that queries [i0, i1) can see: [0, n1) and then t0, t0 + 1, ... ; n = how many in all.
+struct KeyTiles { int n1, t0, n; };
+__device__ __forceinline__ KeyTiles key_tiles(const WindowParams& p, int i0, int i1, int len, int BK) {
+    KeyTiles r = {0, 0, 0};
+    if (i0 >= len) return r;
+    int a = 0, e = len;
+    if (p.causal) e = min(e, i1);
+    int s = 0;                                           // one past the last sink that can be seen
+    if (p.w >= 0) {
+        a = max(0, i0 - p.w);
+        s = min(p.S, e);
+        e = (int)min((long)e, (long)i1 + p.w);
+    }
+    r.t0 = a / BK;
+    const int t1 = (e + BK - 1) / BK, ts = (s + BK - 1) / BK;
+    r.n1 = min(ts, r.t0);
+    r.n = r.n1 + max(t1, ts) - r.t0;                     // sinks past the window's end follow its tiles
+    return r;
+}
+__device__ __forceinline__ int key_tile(const KeyTiles& t, int it) { return it < t.n1 ? it : t.t0 + it - t.n1; }
+
+// Which keys query i sees: j - lo <= span (unsigned), or j < s.
+struct RowRange { int lo; unsigned span; int s; };
+__device__ __forceinline__ RowRange row_range(const WindowParams& p, int i, int len) {
+    RowRange r = {1 << 30, 0u, 0};
+    if (i >= len) return r;
+    const int e = p.causal ? i : len - 1;
+    if (p.w < 0) { r.lo = 0; r.span = (unsigned)e; return r; }
+    r.lo = i - p.w;                                      // p.w < N: no overflow
+    r.span = (unsigned)(min(e, i + p.w) - r.lo);
+    r.s = min(p.S, e + 1);
+    return r;
+}
+// for a wave's queries [i, i + 32) and keys [j0, j0 + BK): 0 nothing visible, 1 some, 2 all
+__device__ __forceinline__ int tile_kind(const WindowParams& p, int i, int j0, int BK, int len) {
+    if (i >= len) return 0;
+    const int j1 = j0 + BK - 1, i1 = i + 31;
+    if (p.causal && j0 > i1) return 0;
+    const bool in = p.w < 0 || (j1 >= i - p.w && j0 <= i1 + p.w);
+    if (!in && j0 >= p.S) return 0;
+    const bool all = (p.w < 0 || (j0 >= i1 - p.w && j1 <= i + p.w) || j1 < p.S) && (!p.causal || j1 <= i) && j1 < len;
+    return all ? 2 : 1;
+}
+
+// ---------------------------------------------------------------------------------------------------------- forward
+template <typename T, int DP, int NW, int BK>
+__global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams p) {
+    using C = WCfg<T, DP>;
+    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * C::LD;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (K tile, V tile)
+    const long id = xcd_order(p.total);
+    if (id < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // order of the work: the group's heads, then query tiles, then (sequence, key head); causal: long rows first
+    const int g = (int)(id % p.G);
+    const long r1 = id / p.G;
+    const int tq = (int)(r1 % p.tiles), bh = (int)(r1 / p.tiles);
+    const int b = bh / p.Hk, hk = bh % p.Hk, h = hk * p.G + g;
+    const int i0 = 32 * NW * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * wave;
+    const int len = p.lengths ? max(0, min(p.lengths[b], p.N)) : p.N;
+    const int i = iw + (lane & 31);
+
+    const T* K = static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh;
+    const T* V = static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh;
+    Frag<T> qf[KD];
+    own_rows<T, DP>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
+
+    const KeyTiles kt = key_tiles(p, i0, i0 + 32 * NW, len, BK);
+    const RowRange rr = row_range(p, i, len);
+    f32x16 o[ND];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+    float m = -INFINITY, l = 0.f;                        // running maximum (log2 domain) and this half-wave's part of the sum
+
+    Stager<T, DP, BK, NT> sk, sv;
+    if (kt.n > 0) {
+        const int j0 = BK * key_tile(kt, 0);
+        sk.load(K, p.k.sn, j0, len, p.dh);
+        sv.load(V, p.v.sn, j0, len, p.dh);
+        sk.store(lds);
+        sv.store(lds + TILE);
+    }
+    for (int it = 0; it < kt.n; ++it) {
+        const T* Ks = lds + (it & 1) * 2 * TILE;
+        const T* Vs = Ks + TILE;
+        __syncthreads();                                 // this tile is staged; the other buffer's readers are done
+        const bool more = it + 1 < kt.n;
+        if (more) {
+            const int j1 = BK * key_tile(kt, it + 1);
+            sk.load(K, p.k.sn, j1, len, p.dh);
+            sv.load(V, p.v.sn, j1, len, p.dh);
+        }
+        const int j0 = BK * key_tile(kt, it);
+        const int kind = tile_kind(p, iw, j0, BK, len);  // the same for the whole wave
+        if (kind) {
+            f32x16 s[NS];
+            float mt = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < KD; ++kk) {
+                    Frag<T> a;
+                    row_frag32<T, C::LD>(a, Ks, 32 * u, kk, lane);
+                    s[u] = mma32(a, qf[kk], s[u]);
+                }
+            }
+            if (kind == 1) {
+#pragma unroll
+                for (int u = 0; u < NS; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = j0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                        const bool ok = (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
+                        s[u][e] = ok ? s[u][e] : -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * p.sc2;
+            // the reference point only has to keep exp2 in range: it moves when a row's maximum has grown by 2^8
+            if (__any(mt > m + 8.f)) {
+                const float mn = fmaxf(m, mt);
+                const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int t = 0; t < ND; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[t][e] *= al;
+            }
+            const float mr = m == -INFINITY ? 0.f : m;
+            if (__any(fabsf(mr) > 16777216.f)) {         // out here the product's rounding, which m has and the fma has not,
+#pragma unroll                                           // would be an exponent of its own
+                for (int u = 0; u < NS; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float x = s[u][e] * p.sc2;
+                        asm("" : "+v"(x));               // two roundings: not to be contracted
+                        s[u][e] = x - mr;
+                    }
+            } else {
+#pragma unroll
+                for (int u = 0; u < NS; ++u)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[u][e] = fmaf(s[u][e], p.sc2, -mr);
+            }
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[u][e] = __builtin_amdgcn_exp2f(s[u][e]);
+                    l += s[u][e];
+                }
+#pragma unroll
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    Frag<T> pf;
+                    acc_frag(pf, s[u], ks);
+#pragma unroll
+                    for (int t = 0; t < ND; ++t) {
+                        Frag<T> a;
+                        col_frag32(a, Vs, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                        o[t] = mma32(a, pf, o[t]);
+                    }
+                }
+        }
+        if (more) {
+            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
+            sk.store(nx);
+            sv.store(nx + TILE);
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    const bool none = i >= len || (m == -INFINITY && l == 0.f);      // nothing visible (a NaN sum stays a NaN)
+    if (p.lse && lane < 32 && i < p.N) p.lse[((long)b * p.Hq + h) * p.N + i] = none ? INFINITY : m + __log2f(l);
+    __syncthreads();
+    put_rows<T, DP>(o, 1.f / l, none, lds + wave * 32 * C::LD, static_cast<T*>(p.out) + ((long)b * p.N * p.Hq + h) * p.dh,
+                    (long)p.Hq * p.dh, iw, p.N, p.dh, lane);
+}
+
+// ------------------------------------------------------------------------------------- backward: dq (and D for the other)
+template <typename T, int DP, int NW, int BK>
+__global__ __launch_bounds__(64 * NW) void window_dq_kernel(const WindowParams p) {
+    using C = WCfg<T, DP>;
+    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * C::LD;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* lds = reinterpret_cast<T*>(smem);
+    const long id = xcd_order(p.total);
+    if (id < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = (int)(id % p.G);
+    const long r1 = id / p.G;
+    const int tq = (int)(r1 % p.tiles), bh = (int)(r1 / p.tiles);
+    const int b = bh / p.Hk, hk = bh % p.Hk, h = hk * p.G + g;
+    const int i0 = 32 * NW * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * wave;
+    const int len = p.lengths ? max(0, min(p.lengths[b], p.N)) : p.N;
+    const int i = iw + (lane & 31);
+
+    const T* K = static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh;
+    const T* V = static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh;
+    Frag<T> qf[KD], df[KD];
+    own_rows<T, DP>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
+    own_rows<T, DP>(df, static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i, len, p.dh, lane);
+    float delta = 0.f, lse = INFINITY;
+    {
+        const T* O = static_cast<const T*>(p.o) + ((long)b * p.N * p.Hq + h) * p.dh;
+#pragma unroll
+        for (int kk = 0; kk < KD; ++kk) {
+            Frag<T> of[1];
+            const int d = 16 * kk + 8 * (lane >> 5);
+            if (i < len && d < p.dh) frag_load(of[0], O + (long)i * p.Hq * p.dh + d);
+            else frag_zero(of[0]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta += frag_get_f(of[0], e) * frag_get_f(df[kk], e);
+        }
+        delta += __shfl_xor(delta, 32, 64);
+        const long at = ((long)b * p.Hq + h) * p.N + i;
+        if (i < len) lse = p.lse[at];
+        if (lane < 32 && i < p.N) p.delta[at] = delta;
+    }
+    const KeyTiles kt = key_tiles(p, i0, i0 + 32 * NW, len, BK);
+    const RowRange rr = row_range(p, i, len);
+    f32x16 dq[ND];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[t][e] = 0.f;
+
+    Stager<T, DP, BK, NT> sk, sv;
+    if (kt.n > 0) {
+        const int j0 = BK * key_tile(kt, 0);
+        sk.load(K, p.k.sn, j0, len, p.dh);
+        sv.load(V, p.v.sn, j0, len, p.dh);
+        sk.store(lds);
+        sv.store(lds + TILE);
+    }
+    for (int it = 0; it < kt.n; ++it) {
+        const T* Ks = lds + (it & 1) * 2 * TILE;
+        const T* Vs = Ks + TILE;
+        __syncthreads();
+        const bool more = it + 1 < kt.n;
+        if (more) {
+            const int j1 = BK * key_tile(kt, it + 1);
+            sk.load(K, p.k.sn, j1, len, p.dh);
+            sv.load(V, p.v.sn, j1, len, p.dh);
+        }
+        const int j0 = BK * key_tile(kt, it);
+        const int kind = tile_kind(p, iw, j0, BK, len);
+        if (kind) {
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+                f32x16 s, dp;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < KD; ++kk) {
+                    Frag<T> a;
+                    row_frag32<T, C::LD>(a, Ks, 32 * u, kk, lane);
+                    s = mma32(a, qf[kk], s);
+                    row_frag32<T, C::LD>(a, Vs, 32 * u, kk, lane);
+                    dp = mma32(a, df[kk], dp);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.sc2, -lse)) * (dp[e] - delta);
+                if (kind == 1) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int j = j0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                        const bool ok = (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
+                        s[e] = ok ? s[e] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    Frag<T> sf;
+                    acc_frag(sf, s, ks);
+#pragma unroll
+                    for (int t = 0; t < ND; ++t) {
+                        Frag<T> a;
+                        col_frag32(a, Ks, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                        dq[t] = mma32(a, sf, dq[t]);
+                    }
+                }
+            }
+        }
+        if (more) {
+            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
+            sk.store(nx);
+            sv.store(nx + TILE);
+        }
+    }
+    __syncthreads();
+    put_rows<T, DP>(dq, p.scale, i >= len, lds + wave * 32 * C::LD, static_cast<T*>(p.out) + ((long)b * p.N * p.Hq + h) * p.dh,
+                    (long)p.Hq * p.dh, iw, p.N, p.dh, lane);
+}
+
+// --------------------------------------------------------------------------------------------- backward: dk and dv
+// A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
+// every head of the group.  SINK: one wave, the 32 keys of a sinks' tile and a share of ALL the query tiles, fp32 partial
+// sums out (window_sink_sum_kernel adds the shares in order).
+template <typename T, int DP, int NW, int BQ, bool SINK>
+__global__ __launch_bounds__(64 * NW) void window_dkv_kernel(const WindowParams p) {
+    using C = WCfg<T, DP>;
+    constexpr int NT = 64 * NW, NS = BQ / 32, KD = DP / 16, ND = DP / 32, TILE = BQ * C::LD;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (Q tile, dO tile), then of BQ (lse, D) each
+    float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
+    const long id = xcd_order(p.total);
+    if (id < 0) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int chunk = 0;
+    long r1 = id;
+    if (SINK) {
+        chunk = (int)(id % p.chunks);
+        r1 = id / p.chunks;
+    }
+    const int tk = (int)(r1 % p.tiles), bh = (int)(r1 / p.tiles);
+    const int b = bh / p.Hk, hk = bh % p.Hk;
+    const int j0 = p.key0 + 32 * NW * tk, jw = j0 + 32 * wave, j = jw + (lane & 31);
+    const int len = p.lengths ? max(0, min(p.lengths[b], p.N)) : p.N;
+
+    Frag<T> kf[KD], vf[KD];
+    own_rows<T, DP>(kf, static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh, p.k.sn, j, len, p.dh, lane);
+    own_rows<T, DP>(vf, static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh, p.v.sn, j, len, p.dh, lane);
+
+    // queries that see key j: i - ilo <= span (unsigned); none for a key past the end
+    int ilo = 1 << 30;
+    unsigned span = 0;
+    if (j < len) {
+        const bool all = p.w < 0 || j < p.S;
+        ilo = p.causal ? j : (all ? 0 : max(0, j - p.w));
+        span = (unsigned)((all ? len - 1 : min(len - 1, j + p.w)) - ilo);
+    }
+    // query tiles [ta, ta + nt) of each of the group's heads
+    int ta = 0, nt = 0;
+    if (j0 < len) {
+        int a = p.causal ? j0 : 0, e = len;
+        if (!SINK && p.w >= 0) {
+            a = max(a, j0 - p.w);
+            e = (int)min((long)e, (long)j0 + 32 * NW + p.w);
+        }
+        ta = a / BQ;
+        nt = (e + BQ - 1) / BQ - ta;
+    }
+    const int items = nt * p.G;
+    const int it0 = SINK ? min(items, chunk * p.per_chunk) : 0, it1 = SINK ? min(items, it0 + p.per_chunk) : items;
+
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dk[t][e] = dv[t][e] = 0.f;
+
+    Stager<T, DP, BQ, NT> sq, sd;
+    float st0 = INFINITY, st1 = 0.f;                     // thread's (lse, D): thread t < BQ holds row t
+    auto fetch = [&](int it) {
+        const int h = hk * p.G + it / nt, i0 = BQ * (ta + it % nt);
+        sq.load(static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i0, len, p.dh);
+        sd.load(static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i0, len, p.dh);
+        st0 = INFINITY;
+        st1 = 0.f;
+        const int i = i0 + (int)threadIdx.x;
+        if ((int)threadIdx.x < BQ && i < len) {
+            const long at = ((long)b * p.Hq + h) * p.N + i;
+            st0 = p.lse[at];
+            st1 = p.delta[at];
+        }
+    };
+    auto put = [&](int it) {
+        T* nx = lds + (it & 1) * 2 * TILE;
+        sq.store(nx);
+        sd.store(nx + TILE);
+        if ((int)threadIdx.x < BQ) {
+            stat[(it & 1) * 2 * BQ + threadIdx.x] = st0;
+            stat[(it & 1) * 2 * BQ + BQ + threadIdx.x] = st1;
+        }
+    };
+    if (it0 < it1) {
+        fetch(it0);
+        put(it0);
+    }
+    for (int it = it0; it < it1; ++it) {
+        const T* Qs = lds + (it & 1) * 2 * TILE;
+        const T* Ds = Qs + TILE;
+        const float* ls = stat + (it & 1) * 2 * BQ;
+        __syncthreads();
+        if (it + 1 < it1) fetch(it + 1);
+        const int i0 = BQ * (ta + it % nt);
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+            const int iu = i0 + 32 * u;
+            const int kind = jw < len ? tile_kind(p, iu, jw, 32, len) : 0;
+            if (!kind) continue;
+            f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KD; ++kk) {
+                Frag<T> a;
+                row_frag32<T, C::LD>(a, Qs, 32 * u, kk, lane);
+                s = mma32(a, kf[kk], s);
+                row_frag32<T, C::LD>(a, Ds, 32 * u, kk, lane);
+                dp = mma32(a, vf[kk], dp);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = 32 * u + 8 * q + 4 * (lane >> 5);
+                const f32x4 L = *reinterpret_cast<const f32x4*>(ls + row), D = *reinterpret_cast<const f32x4*>(ls + BQ + row);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float pe = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], p.sc2, -L[e]));
+                    float se = pe * (dp[4 * q + e] - D[e]);
+                    if (kind == 1) {
+                        const bool ok = (unsigned)(i0 + row + e - ilo) <= span;
+                        pe = ok ? pe : 0.f;
+                        se = ok ? se : 0.f;
+                    }
+                    s[4 * q + e] = pe;
+                    dp[4 * q + e] = se;
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                Frag<T> pf, sf;
+                acc_frag(pf, s, ks);
+                acc_frag(sf, dp, ks);
+#pragma unroll
+                for (int t = 0; t < ND; ++t) {
+                    Frag<T> a;
+                    col_frag32(a, Ds, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                    dv[t] = mma32(a, pf, dv[t]);
+                    col_frag32(a, Qs, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                    dk[t] = mma32(a, sf, dk[t]);
+                }
+            }
+        }
+        if (it + 1 < it1) put(it + 1);
+    }
+    if (SINK) {
+        float* o = p.part + id * 2 * DP * 32;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int d = 32 * t + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                o[d * 32 + (lane & 31)] = dk[t][e];
+                o[(DP + d) * 32 + (lane & 31)] = dv[t][e];
+            }
+        return;
+    }
+    __syncthreads();
+    T* mine = lds + wave * 32 * C::LD;
+    const long at = ((long)b * p.N * p.Hk + hk) * p.dh, ldg = (long)p.Hk * p.dh;
+    put_rows<T, DP>(dk, p.scale, j >= len, mine, static_cast<T*>(p.dk) + at, ldg, jw, p.N, p.dh, lane);
+    put_rows<T, DP>(dv, 1.f, j >= len, mine, static_cast<T*>(p.dv) + at, ldg, jw, p.N, p.dh, lane);
+}
+
+// rows of the sinks' tiles: the shares' sum, rounded once.  One workgroup a (sequence, key head, tile).
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void window_sink_sum_kernel(const WindowParams p) {
+    __shared__ float t[32][DP + 1];
+    const int tk = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles;
+    const int b = bh / p.Hk, hk = bh % p.Hk;
+    const float* part = p.part + (long)blockIdx.x * p.chunks * 2 * DP * 32;
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        T* out = static_cast<T*>(which ? p.dv : p.dk);
+        for (int e = threadIdx.x; e < DP * 32; e += 256) {
+            float s = 0.f;
+            for (int c = 0; c < p.chunks; ++c) s += part[((long)c * 2 + which) * DP * 32 + e];
+            t[e & 31][e >> 5] = which ? s : s * p.scale;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < DP * 32; e += 256) {
+            const int r = e / DP, d = e % DP, j = 32 * tk + r;
+            if (j < p.N && d < p.dh) out[(((long)b * p.N + j) * p.Hk + hk) * p.dh + d] = (T)t[r][d];
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace vitk
+
+using namespace vitk;
+
+namespace {
+
+struct Plan {                  // tiles of one call
+    int dp;                    // staged head width: 32, 64, 96 or 128
+    int nwq, nwk;              // waves of a query / key workgroup
+    int sink_keys;             // keys that the sinks' launch takes (a multiple of 32, 0: none)
+    int chunks, per_chunk;
+};
+constexpr int SINK_BQ = 32;
+
+// Fewer, larger workgroups read K and V fewer times; they are halved where the large ones would leave CUs without work.
+int waves_for(long rows_tiles_of_128) { return rows_tiles_of_128 >= 512 ? 4 : 2; }
+
+Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S) {
+    Plan pl;
+    pl.dp = (dh + 31) / 32 * 32;
+    pl.nwq = waves_for((long)B * Hq * ((N + 127) / 128));
+    pl.nwk = waves_for((long)B * Hk * ((N + 127) / 128));
+    pl.sink_keys = w >= 0 && S > 0 ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
+    pl.chunks = pl.per_chunk = 0;
+    if (pl.sink_keys) {
+        // about 1024 one-wave workgroups, at least 4 query tiles each
+        const long items = (long)((N + SINK_BQ - 1) / SINK_BQ) * (Hq / Hk), sets = (long)B * Hk * (pl.sink_keys / 32);
+        long want = (1024 + sets - 1) / sets;
+        long per = (items + want - 1) / want;
+        if (per < 4) per = 4;
+        pl.per_chunk = (int)per;
+        pl.chunks = (int)((items + per - 1) / per);
+    }
+    return pl;
+}
+long part_floats(const Plan& pl, int B, int Hk) { return (long)B * Hk * (pl.sink_keys / 32) * pl.chunks * 2 * pl.dp * 32; }
+
+int check_window(const char* what, int dtype, int B, int N, int Hq, int Hk, int dh, float scale, int sinks) {
+    VITK_CHECK_ARG(dtype == VITK_F32 || dtype == VITK_BF16, "%s: bad dtype %d", what, dtype);
+    VITK_CHECK_ARG(B >= 0 && N >= 0 && N < (1 << 28) && Hq >= 1 && Hk >= 1, "%s: bad shape B=%d N=%d Hq=%d Hk=%d", what, B, N, Hq, Hk);
+    VITK_CHECK_ARG(Hq % Hk == 0, "%s: %d query heads are no multiple of %d key heads", what, Hq, Hk);
+    VITK_CHECK_ARG(dh >= 8 && dh <= 128 && dh % 8 == 0, "%s: head width %d must be a multiple of 8 up to 128", what, dh);
+    VITK_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: the scale must be positive and finite", what);
+    VITK_CHECK_ARG(sinks >= 0, "%s: bad number of sinks %d", what, sinks);
+    return VITK_OK;
+}
+int check_view(const char* what, const char* name, const View& v, int dtype) {
+    const int per = dtype == VITK_F32 ? 4 : 8;
+    VITK_CHECK_ARG(v.p && (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.sb % per == 0 && v.sn % per == 0 && v.sh % per == 0,
+                   "%s: %s must be 16-byte aligned, its strides too", what, name);
+    return VITK_OK;
+}
+void fill_params(WindowParams& p, int B, int N, int Hq, int Hk, int dh, int w, int S, int causal, float scale, const int* lengths) {
+    p.lengths = lengths;
+    p.B = B; p.N = N; p.Hq = Hq; p.Hk = Hk; p.G = Hq / Hk; p.dh = dh;
+    p.w = w < 0 || w >= N - 1 ? -1 : w;                  // a window that covers the sequence is no window
+    p.S = p.w < 0 ? 0 : (S < N ? S : N);
+    p.causal = causal != 0;
+    p.scale = scale;
+    p.sc2 = scale * 1.4426950408889634f;
+}
+unsigned xcd_grid(long total) { return (unsigned)((total + 7) / 8 * 8); }
+
+template <typename T, int DP, int NW> int run_fwd(WindowParams p, hipStream_t st) {
+    constexpr int BK = sizeof(T) == 2 ? 64 : 32;
+    p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
+    p.total = (long)p.B * p.Hq * p.tiles;
+    const size_t tiles = 4 * BK * WCfg<T, DP>::LD * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
+    const size_t lds = tiles > rows ? tiles : rows;
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK>), lds);
+    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+    return VITK_OK;
+}
+template <typename T, int DP, int NW> void run_dq(WindowParams p, hipStream_t st) {
+    constexpr int BK = sizeof(T) == 2 ? 64 : 32;
+    p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
+    p.total = (long)p.B * p.Hq * p.tiles;
+    const size_t tiles = 4 * BK * WCfg<T, DP>::LD * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
+    const size_t lds = tiles > rows ? tiles : rows;
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK>), lds);
+    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+}
+template <typename T, int DP, int NW, int BQ, bool SINK> void run_dkv(WindowParams p, int tiles, hipStream_t st) {
+    p.tiles = tiles;
+    p.total = (long)p.B * p.Hk * tiles * (SINK ? p.chunks : 1);
+    const size_t tl = 4 * BQ * WCfg<T, DP>::LD * sizeof(T) + 4 * BQ * sizeof(float), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
+    const size_t lds = tl > rows ? tl : rows;
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK>), lds);
+    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+}
+template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
+    constexpr int BQ = sizeof(T) == 2 ? 64 : 32;
+    p.out = dq;
+    if (pl.nwq == 4) run_dq<T, DP, 4>(p, st);
+    else run_dq<T, DP, 2>(p, st);
+    if (pl.sink_keys) {
+        WindowParams s = p;
+        s.key0 = 0;
+        s.chunks = pl.chunks;
+        s.per_chunk = pl.per_chunk;
+        run_dkv<T, DP, 1, SINK_BQ, true>(s, pl.sink_keys / 32, st);
+        s.tiles = pl.sink_keys / 32;
+        hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles)), dim3(256), 0, st, s);
+    }
+    p.key0 = pl.sink_keys;
+    const int rest = p.N - pl.sink_keys;
+    if (rest > 0) {
+        if (pl.nwk == 4) run_dkv<T, DP, 4, BQ, false>(p, (rest + 127) / 128, st);
+        else run_dkv<T, DP, 2, BQ, false>(p, (rest + 63) / 64, st);
+    }
+}
+
+}  // namespace
+
+extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
+                                    const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
+                                    int window, int sinks, int causal, const int* lengths, void* out, float* lse, hipStream_t stream) {
+    const char* what = "vitk_window_attn_fwd";
+    if (int e = check_window(what, dtype, B, N, Hq, Hk, dh, scale, sinks)) return e;
+    if (B == 0 || N == 0) return VITK_OK;
+    WindowParams p = {};
+    p.q = View{q, qb, qn, qh};
+    p.k = View{k, kb, kn, kh};
+    p.v = View{v, vb, vn, vh};
+    if (int e = check_view(what, "q", p.q, dtype)) return e;
+    if (int e = check_view(what, "k", p.k, dtype)) return e;
+    if (int e = check_view(what, "v", p.v, dtype)) return e;
+    VITK_CHECK_ARG(out && (reinterpret_cast<uintptr_t>(out) & 15) == 0, "%s: out must be 16-byte aligned", what);
+    fill_params(p, B, N, Hq, Hk, dh, window, sinks, causal, scale, lengths);
+    p.out = out;
+    p.lse = lse;
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    VITK_CHECK_ARG((long)B * Hq * ((N + 63) / 64) < (1L << 30), "%s: too many tiles for one call", what);
+#define GO(T, D) if (pl.nwq == 4) run_fwd<T, D, 4>(p, stream); else run_fwd<T, D, 2>(p, stream)
+#define BY_DP(T) switch (pl.dp) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 96: GO(T, 96); break; default: GO(T, 128); break; }
+    if (dtype == VITK_BF16) { BY_DP(__bf16) }
+    else { BY_DP(float) }
+#undef GO
+    VITK_CHECK_LAUNCH(what);
+    return VITK_OK;
+}
+
+extern "C" long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, int Hq, int Hk, int dh, int window, int sinks) {
+    if (B <= 0 || N <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || dh < 8 || dh > 128 || sinks < 0) return 0;
+    WindowParams p = {};
+    fill_params(p, B, N, Hq, Hk, dh, window, sinks, 0, 1.f, nullptr);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    return ((long)B * Hq * N + 3) / 4 * 16 + part_floats(pl, B, Hk) * 4;
+}
+
+extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
+                                    const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
+                                    int window, int sinks, int causal, const int* lengths, const void* out, const float* lse,
+                                    const void* dout, long ob, long on, long oh, void* dq, void* dk, void* dv, void* workspace,
+                                    hipStream_t stream) {
+    const char* what = "vitk_window_attn_bwd";
+    if (int e = check_window(what, dtype, B, N, Hq, Hk, dh, scale, sinks)) return e;
+    if (B == 0 || N == 0) return VITK_OK;
+    WindowParams p = {};
+    p.q = View{q, qb, qn, qh};
+    p.k = View{k, kb, kn, kh};
+    p.v = View{v, vb, vn, vh};
+    p.dout = View{dout, ob, on, oh};
+    if (int e = check_view(what, "q", p.q, dtype)) return e;
+    if (int e = check_view(what, "k", p.k, dtype)) return e;
+    if (int e = check_view(what, "v", p.v, dtype)) return e;
+    if (int e = check_view(what, "dout", p.dout, dtype)) return e;
+    VITK_CHECK_ARG(out && lse && dq && dk && dv && workspace, "%s: null pointer", what);
+    VITK_CHECK_ARG(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) |
+                     reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
+                   "%s: out, dq, dk, dv and the workspace must be 16-byte aligned", what);
+    VITK_CHECK_ARG((long)B * Hq * ((N + 63) / 64) < (1L << 30), "%s: too many tiles for one call", what);
+    fill_params(p, B, N, Hq, Hk, dh, window, sinks, causal, scale, lengths);
+    p.o = out;
+    p.lse = const_cast<float*>(lse);
+    p.delta = static_cast<float*>(workspace);
+    p.part = p.delta + ((long)B * Hq * N + 3) / 4 * 4;
+    p.dk = dk;
+    p.dv = dv;
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+#define GO(T, D) run_bwd<T, D>(p, pl, dq, stream)
+    if (dtype == VITK_BF16) { BY_DP(__bf16) }
+    else { BY_DP(float) }
+#undef GO
+#undef BY_DP
+    VITK_CHECK_LAUNCH(what);
+    return VITK_OK;
+}

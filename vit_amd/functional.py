@@ -9,10 +9,12 @@ type: fp32 runs the exact f32 MFMA path (parity to 1e-5), bf16 keeps a bf16 shad
 (refreshed when the parameter's version counter moves) and bf16 activations with fp32
 accumulation, statistics, softmax, bias, LayerNorm affine and all parameter gradients.
 """
+import math
 import os
 import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from . import dropout as VD
@@ -1048,3 +1050,153 @@ def label_smoothing_ce(logits, target, smoothing=0.1):
     if target.dtype != torch.int64:
         target = target.long()
     return LabelSmoothingCEFn.apply(logits, target.contiguous(), float(smoothing))
+
+
+# ------------------------------------------------------------------ long sequences: rotary positions, window attention
+def rotary_frequencies(dim, base=10000.0, scaling=None):
+    """(frequencies of the dim / 2 pairs, factor of cos and sin), in double precision.  ``scaling``: None, or a dict with
+    ``type`` and ``factor`` (how many times longer the context is than the trained one):
+
+    'linear'  positions divided by the factor (position interpolation)
+    'ntk'     base * factor^(dim / (dim - 2)): the slowest pair is interpolated, the fastest left alone
+    'yarn'    by parts (YaRN): pairs that turn more than ``beta_fast`` (32) times over the ``original`` length keep their
+              frequency, those under ``beta_slow`` (1) are interpolated, a ramp in between; cos and sin times 0.1 ln(factor) + 1
+    """
+    if dim < 2 or dim % 2:
+        raise ValueError(f'rotary: the rotated width {dim} must be even and positive')
+    if not base > 0:
+        raise ValueError('rotary: the base must be positive')
+    kind = None if scaling is None else scaling.get('type')
+    known = {None: (), 'linear': ('factor',), 'ntk': ('factor',), 'yarn': ('factor', 'original', 'beta_fast', 'beta_slow')}
+    if scaling is not None and (kind is None or kind not in known or set(scaling) - {'type'} - set(known[kind])):
+        raise ValueError(f'rotary: unknown scaling {scaling!r}')
+    f = 1.0
+    if kind is not None:
+        f = float(scaling.get('factor', 0))
+        if not 0 < f < math.inf:
+            raise ValueError('rotary: scaling needs a positive factor')
+    if kind == 'ntk' and dim > 2:
+        base = base * f ** (dim / (dim - 2))
+    freqs = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if kind == 'linear':
+        freqs = [w / f for w in freqs]
+    if kind == 'yarn':
+        n, fast, slow = float(scaling.get('original', 0)), float(scaling.get('beta_fast', 32)), float(scaling.get('beta_slow', 1))
+        if not n > 0 or not fast > slow:
+            raise ValueError("rotary: 'yarn' needs the original length, and beta_fast > beta_slow")
+        ramp = [min(1.0, max(0.0, (n * w / (2 * math.pi) - slow) / (fast - slow))) for w in freqs]
+        return [w * ((1 - r) / f + r) for w, r in zip(freqs, ramp)], (0.1 * math.log(f) + 1.0 if f > 1 else 1.0)
+    return freqs, 1.0
+
+
+def rotary_table(positions, dim, base=10000.0, scaling=None):
+    """(cos, sin) of every position and pair, fp32 [P, dim / 2, 2], for ``rotary`` / ``qk_norm_rotary``.  ``positions`` [P], or
+    [P, A] for A axes (rows and columns of a patch grid: the pairs are shared evenly, axis 0 first); integers or floats
+    on the GPU.  Angles and their sines are computed in 64 bits: far positions keep theirs."""
+    axes = positions.shape[1] if positions.dim() == 2 else 1
+    if axes < 1 or dim % (2 * axes):
+        raise ValueError(f'rotary_table: a rotated width of {dim} is no whole number of pairs over {axes} axes')
+    freqs, mul = rotary_frequencies(dim // axes, base, scaling)
+    return ops.rotary_table(positions, freqs, mul)
+
+
+def _unit_heads(t):
+    """``t`` with contiguous heads (a copy where they are not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+class RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, table, pos, offset, interleaved):
+        ctx.save_for_backward(table, pos)
+        ctx.cfg = (offset, interleaved)
+        return ops.rotary(_unit_heads(x), table, pos, offset, interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        table, pos = ctx.saved_tensors
+        offset, interleaved = ctx.cfg
+        return ops.rotary(_unit_heads(dy), table, pos, offset, interleaved, inverse=True), None, None, None, None
+
+
+def rotary(x, table, pos=None, offset=0, interleaved=False):
+    """Rotary positions on x [B, N, H, dh] (any strides): the first 2 * table.shape[1] elements of every head are turned, the
+    rest is copied.  Pair i is (i, i + half), or (2i, 2i + 1) when ``interleaved``.  Token (b, n) takes table row pos[b, n] (int32
+    / int64 [B, N]), or offset + n.  A pos outside the table gives NaN.  Differentiable in x."""
+    return RotaryFn.apply(x, table, pos, offset, interleaved)
+
+
+class QkNormRotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
+        q, k = _unit_heads(q), _unit_heads(k)
+        ctx.save_for_backward(q, k, gamma_q, gamma_k, table, pos)
+        ctx.cfg = (offset, eps, interleaved)
+        return ops.qk_norm_rotary_fwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, gamma_q, gamma_k, table, pos = ctx.saved_tensors
+        offset, eps, interleaved = ctx.cfg
+        want = ctx.needs_input_grad
+        dq, dk, dgq, dgk = ops.qk_norm_rotary_bwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved, _unit_heads(dq),
+                                                  _unit_heads(dk), want[2], want[3])
+        return dq, dk, dgq, dgk, None, None, None, None, None
+
+
+def qk_norm_rotary(q, k, gamma_q, gamma_k, table=None, pos=None, offset=0, eps=1e-6, interleaved=False):
+    """RMS norm of every head of q [B, N, Hq, dh] and k [B, N, Hk, dh], times gamma (fp32 [dh] or None), and the rotary turn of
+    ``rotary`` (table None: none) in one pass: (q', k'), contiguous.  dh <= 128.  Differentiable in q, k and the gammas; the
+    gammas' sums run in a fixed order."""
+    return QkNormRotaryFn.apply(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
+
+
+class WindowAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, causal, scale, lengths):
+        q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
+        train = any(ctx.needs_input_grad[:3])
+        out, lse = ops.window_attn_fwd(q, k, v, window, sinks, causal, scale, lengths, want_lse=train)
+        if train:
+            ctx.save_for_backward(q, k, v, out, lse, lengths)
+            ctx.cfg = (window, sinks, causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        window, sinks, causal, scale = ctx.cfg
+        dq, dk, dv = ops.window_attn_bwd(q, k, v, window, sinks, causal, scale, lengths, out, lse, ops._aligned_heads(dout))
+        return dq, dk, dv, None, None, None, None, None
+
+
+def window_attention(q, k, v, window, sinks=0, causal=False, scale=None, lengths=None):
+    """Attention of q [B, N, Hq, dh] over k, v [B, N, Hk, dh] (any strides; Hq a multiple of Hk, dh a multiple of 8 up to 128):
+    query i sees the keys j with |i - j| <= window, and the first ``sinks`` keys (class / register tokens) wherever it is;
+    ``causal``: of those only j <= i.  window < 0: every key.  ``lengths`` (int32 [B]): tokens of each padded sequence; rows past
+    it are not read, and their outputs and gradients are 0.  scale: dh^-0.5 unless given (positive).  out [B, N, Hq, dh],
+    contiguous."""
+    return WindowAttentionFn.apply(q, k, v, window, sinks, causal, q.shape[-1] ** -0.5 if scale is None else scale, lengths)
+
+
+def window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks=0, scale=None):
+    """The causal window attention of one new token a sequence: q [B, Hq, dh], k and v [B, Hk, dh]; out [B, Hq, dh].  k and v go
+    into the ring caches [B, Hk, slots, dh] in place: token p into slot p for p < sinks, else sinks + (p - sinks) % (slots -
+    sinks); slots >= sinks + window + 1.  ``lengths`` (int32 [B]) are the tokens before the new one and are not advanced here;
+    < 0 leaves a sequence out (its row is 0, its cache untouched).  window < 0: nothing is overwritten; a sequence whose
+    cache is full gets NaN and writes nothing.  No backward."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise RuntimeError('window_decode has no backward: call it under torch.no_grad()')
+    out = ops.window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks, q.shape[-1] ** -0.5 if scale is None else scale)
+    torch.autograd.graph.increment_version((k_cache, v_cache))
+    return out
+
+
+def window_cache_fill(k, v, k_cache, v_cache, sinks=0, lengths=None):
+    """The k and v [B, N, Hk, dh] of whole prompts (``lengths``: int32 [B] of padded ones) into the empty ring caches of
+    ``window_decode``, in place: every slot takes the last token that belongs in it, the others are left as they are."""
+    ops.window_cache_fill(k, v, k_cache, v_cache, sinks, lengths)
+    torch.autograd.graph.increment_version((k_cache, v_cache))

@@ -506,3 +506,235 @@ def ce_smooth_bwd(logits, target, smoothing, lse, gout):
                                   lse.data_ptr(), gout.data_ptr(), d.data_ptr(), C, _stream())
     check(st, 'vitk_ce_smooth_bwd')
     return d
+
+
+# ------------------------------------------------------------------ long sequences: rotary positions, window attention
+def _req_here(*ts):
+    """Every tensor on the current device, where the launch goes."""
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in ts:
+        if t is not None and not (t.is_cuda and t.get_device() == dev):
+            raise _lib.VitkError('vit_amd ops need tensors on the current GPU (there is no CPU path)')
+
+
+def _heads(t, what):
+    """Shape and strides of a [B, N, H, dh] view whose last dim is contiguous."""
+    if t.dim() != 4 or t.shape[3] > 1 and t.stride(3) != 1 and t.numel():
+        raise ValueError(f'{what}: need [B, N, H, dh] with contiguous heads, got {tuple(t.shape)} strides {t.stride()}')
+    return t.shape, t.stride()
+
+
+def _aligned_heads(t):
+    """16-byte aligned rows, as the attention kernels read them: ``t`` itself, or a copy."""
+    per = 16 // t.element_size()
+    s = t.stride()
+    if s[-1] == 1 and t.data_ptr() % 16 == 0 and not any(x % per for x in s[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+_POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+
+
+def rotary_table(positions, freqs, mul=1.0):
+    """fp32 [P, A * len(freqs), 2] of mul * (cos, sin)(positions[p, a] * freqs[i]), angles in 64 bits.  ``positions``: [P] or
+    [P, A] on the GPU (int32, int64, float32 or float64); ``freqs``: floats on the host."""
+    import ctypes
+    _req_here(positions)
+    if positions.dim() not in (1, 2) or positions.dtype not in _POS_KIND:
+        raise ValueError('rotary_table: positions must be [P] or [P, axes], int32 / int64 / float32 / float64')
+    if not 1 <= len(freqs) <= 128:
+        raise ValueError('rotary_table: 1 to 128 frequencies an axis')
+    axes = 1 if positions.dim() == 1 else positions.shape[1]
+    if axes < 1:
+        raise ValueError('rotary_table: positions without an axis')
+    positions = positions.contiguous()
+    P, pairs = positions.shape[0], axes * len(freqs)
+    table = torch.empty(P, pairs, 2, device=positions.device, dtype=torch.float32)
+    arr = (ctypes.c_double * len(freqs))(*[float(f) for f in freqs])
+    check(lib().vitk_rotary_table(_POS_KIND[positions.dtype], axes, P, positions.data_ptr(), pairs,
+                                  ctypes.cast(arr, ctypes.c_void_p), float(mul), table.data_ptr(), _stream()), 'vitk_rotary_table')
+    return table
+
+
+def _turn_args(what, B, N, dh, table, pos, offset):
+    """(table pointer, rows, rotated width, ids pointer, ids are int64, offset) of a call over [B, N] tokens."""
+    if table is None:
+        if pos is not None or offset:
+            raise ValueError(f'{what}: positions without a table')
+        return 0, 0, 0, 0, 0, 0
+    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise ValueError(f'{what}: the table must be contiguous fp32 [rows, pairs, 2] (rotary_table)')
+    if 2 * table.shape[1] > dh:
+        raise ValueError(f'{what}: the table turns {2 * table.shape[1]} elements of heads of {dh}')
+    if pos is None:
+        return table.data_ptr(), table.shape[0], 2 * table.shape[1], 0, 0, int(offset)
+    if offset:
+        raise ValueError(f'{what}: give pos or offset, not both')
+    if tuple(pos.shape) != (B, N) or pos.dtype not in (torch.int32, torch.int64) or not pos.is_contiguous():
+        raise ValueError(f'{what}: pos must be contiguous int32 / int64 [B, N]')
+    return table.data_ptr(), table.shape[0], 2 * table.shape[1], pos.data_ptr(), int(pos.dtype == torch.int64), 0
+
+
+def rotary(x, table, pos=None, offset=0, interleaved=False, inverse=False):
+    """Rotary positions on x [B, N, H, dh] (any strides, contiguous heads): a new contiguous tensor.  Token (b, n) takes table row
+    pos[b, n], or offset + n; ids outside the table give NaN.  ``inverse``: the adjoint."""
+    _req_here(x, table, pos)
+    (B, N, H, dh), st = _heads(x, 'rotary x')
+    tp, rows, rot, ids, ids64, offset = _turn_args('rotary', B, N, dh, table, pos, offset)
+    if table is None:
+        raise ValueError('rotary: no table')
+    y = torch.empty(B, N, H, dh, device=x.device, dtype=x.dtype)
+    check(lib().vitk_rotary(_dt(x), int(inverse), int(interleaved), B, N, H, dh, x.data_ptr(), st[0], st[1], st[2], tp, rows, rot,
+                            ids, ids64, offset, y.data_ptr(), _stream()), 'vitk_rotary')
+    return y
+
+
+def _check_qk(q, k, gamma_q, gamma_k):
+    (B, N, Hq, dh), sq = _heads(q, 'qk_norm_rotary q')
+    shape, sk = _heads(k, 'qk_norm_rotary k')
+    if k.dtype != q.dtype or (shape[0], shape[1], shape[3]) != (B, N, dh):
+        raise ValueError('qk_norm_rotary: q and k must share B, N, dh and their type')
+    for g in (gamma_q, gamma_k):
+        if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (dh,) or not g.is_contiguous()):
+            raise ValueError('qk_norm_rotary: gamma must be contiguous fp32 [dh]')
+    return B, N, Hq, shape[2], dh, sq, sk
+
+
+def qk_norm_rotary_fwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
+    _req_here(q, k, gamma_q, gamma_k, table, pos)
+    B, N, Hq, Hk, dh, sq, sk = _check_qk(q, k, gamma_q, gamma_k)
+    turn = _turn_args('qk_norm_rotary', B, N, dh, table, pos, offset)
+    yq = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
+    yk = torch.empty(B, N, Hk, dh, device=q.device, dtype=q.dtype)
+    check(lib().vitk_qk_norm_rotary_fwd(_dt(q), int(interleaved), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2],
+                                        k.data_ptr(), sk[0], sk[1], sk[2], _ptr(gamma_q), _ptr(gamma_k), float(eps), *turn,
+                                        yq.data_ptr(), yk.data_ptr(), _stream()), 'vitk_qk_norm_rotary_fwd')
+    return yq, yk
+
+
+def qk_norm_rotary_bwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved, dyq, dyk, want_dgq, want_dgk):
+    """(dq, dk, dgamma_q, dgamma_k); a gamma gradient that is not wanted is None."""
+    _req_here(q, k, gamma_q, gamma_k, table, pos, dyq, dyk)
+    B, N, Hq, Hk, dh, sq, sk = _check_qk(q, k, gamma_q, gamma_k)
+    turn = _turn_args('qk_norm_rotary', B, N, dh, table, pos, offset)
+    (s1, gq), (s2, gk) = _heads(dyq, 'qk_norm_rotary dq'), _heads(dyk, 'qk_norm_rotary dk')
+    if s1 != q.shape or s2 != k.shape or dyq.dtype != q.dtype or dyk.dtype != q.dtype:
+        raise ValueError('qk_norm_rotary: the gradients must match the outputs')
+    dq = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
+    dk = torch.empty(B, N, Hk, dh, device=q.device, dtype=q.dtype)
+    dgq = torch.empty(dh, device=q.device, dtype=torch.float32) if want_dgq else None
+    dgk = torch.empty(dh, device=q.device, dtype=torch.float32) if want_dgk else None
+    ws = None
+    if want_dgq or want_dgk:
+        ws = torch.empty(lib().vitk_qk_norm_rotary_bwd_workspace_bytes(dh), device=q.device, dtype=torch.uint8)
+    check(lib().vitk_qk_norm_rotary_bwd(_dt(q), int(interleaved), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2],
+                                        k.data_ptr(), sk[0], sk[1], sk[2], _ptr(gamma_q), _ptr(gamma_k), float(eps), *turn,
+                                        dyq.data_ptr(), gq[0], gq[1], gq[2], dyk.data_ptr(), gk[0], gk[1], gk[2],
+                                        dq.data_ptr(), dk.data_ptr(), _ptr(dgq), _ptr(dgk), _ptr(ws), _stream()),
+          'vitk_qk_norm_rotary_bwd')
+    return dq, dk, dgq, dgk
+
+
+def _check_window(q, k, v, window, sinks, lengths):
+    (B, N, Hq, dh), sq = _heads(q, 'window_attention q')
+    shape, sk = _heads(k, 'window_attention k')
+    shape_v, sv = _heads(v, 'window_attention v')
+    if shape != shape_v or (shape[0], shape[1], shape[3]) != (B, N, dh) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('window_attention: q, k and v must share B, N, dh and their type, k and v their heads')
+    Hk = shape[2]
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError(f'window_attention: {Hq} query heads are no multiple of {Hk} key heads')
+    if dh % 8 or not 8 <= dh <= 128:
+        raise ValueError(f'window_attention: head width {dh} must be a multiple of 8 up to 128')
+    if sinks < 0:
+        raise ValueError('window_attention: sinks must not be negative')
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
+        raise ValueError('window_attention: lengths must be contiguous int32 [B]')
+    return B, N, Hq, Hk, dh, sq, sk, sv
+
+
+def _i32(n):
+    """An int argument of the C ABI: a count past its range means the same as the range's end."""
+    return max(-1, min(int(n), 2 ** 31 - 1))
+
+
+def window_attn_fwd(q, k, v, window, sinks, causal, scale, lengths, want_lse=True):
+    """(out [B, N, Hq, dh], lse [B, Hq, N] in log2 or None)."""
+    _req_here(q, k, v, lengths)
+    B, N, Hq, Hk, dh, sq, sk, sv = _check_window(q, k, v, window, sinks, lengths)
+    out = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
+    lse = torch.empty(B, Hq, N, device=q.device, dtype=torch.float32) if want_lse else None
+    check(lib().vitk_window_attn_fwd(_dt(q), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
+                                     v.data_ptr(), sv[0], sv[1], sv[2], float(scale), _i32(window), _i32(sinks), int(causal),
+                                     _ptr(lengths), out.data_ptr(), _ptr(lse), _stream()), 'vitk_window_attn_fwd')
+    return out, lse
+
+
+def window_attn_bwd(q, k, v, window, sinks, causal, scale, lengths, out, lse, dout):
+    """(dq, dk, dv), contiguous."""
+    _req_here(q, k, v, lengths, out, lse, dout)
+    B, N, Hq, Hk, dh, sq, sk, sv = _check_window(q, k, v, window, sinks, lengths)
+    shape, so = _heads(dout, 'window_attention dout')
+    if shape != q.shape or dout.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError('window_attention: out / dout must match q')
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hq, N) or not lse.is_contiguous():
+        raise ValueError('window_attention: lse must be contiguous fp32 [B, Hq, N]')
+    window, sinks = _i32(window), _i32(sinks)
+    dq = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
+    dk, dv = (torch.empty(B, N, Hk, dh, device=q.device, dtype=q.dtype) for _ in range(2))
+    ws = torch.empty(lib().vitk_window_attn_bwd_workspace_bytes(_dt(q), B, N, Hq, Hk, dh, window, sinks), device=q.device,
+                     dtype=torch.uint8)
+    check(lib().vitk_window_attn_bwd(_dt(q), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
+                                     v.data_ptr(), sv[0], sv[1], sv[2], float(scale), window, sinks, int(causal), _ptr(lengths),
+                                     out.data_ptr(), lse.data_ptr(), dout.data_ptr(), so[0], so[1], so[2], dq.data_ptr(),
+                                     dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), _stream()), 'vitk_window_attn_bwd')
+    return dq, dk, dv
+
+
+def _check_cache(what, k_cache, v_cache, B, Hk, dh, dtype, lengths):
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or (k_cache.shape[0], k_cache.shape[1], k_cache.shape[3]) != (B, Hk, dh) \
+            or k_cache.dtype != dtype or v_cache.dtype != dtype or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f'{what}: the caches must be contiguous [B, Hk, slots, dh] of the type of k and v')
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
+        raise ValueError(f'{what}: lengths must be contiguous int32 [B]')
+    return k_cache.shape[2]
+
+
+def window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks, scale):
+    """One new token a sequence: its k / v [B, Hk, dh] into the ring caches (in place), its q [B, Hq, dh] over what is visible:
+    out [B, Hq, dh]."""
+    _req_here(q, k, v, k_cache, v_cache, lengths)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] \
+            or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('window_decode: q [B, Hq, dh], k and v [B, Hk, dh] of one type expected')
+    if lengths is None:
+        raise ValueError('window_decode: lengths are needed')
+    B, Hq, dh = q.shape
+    Hk = k.shape[1]
+    C = _check_cache('window_decode', k_cache, v_cache, B, Hk, dh, q.dtype, lengths)
+    q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
+    window, sinks = _i32(window), int(sinks)
+    L, dt = lib(), _dt(q)
+    out = torch.empty(B, Hq, dh, device=q.device, dtype=q.dtype)
+    need = L.vitk_window_decode_workspace_bytes(dt, B, Hq, Hk, dh, C, window, sinks)
+    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+    check(L.vitk_window_decode(dt, B, Hq, Hk, dh, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                               v.data_ptr(), v.stride(0), v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), C,
+                               lengths.data_ptr(), float(scale), window, sinks, out.data_ptr(), _ptr(ws), _stream()),
+          'vitk_window_decode')
+    return out
+
+
+def window_cache_fill(k, v, k_cache, v_cache, sinks, lengths=None):
+    """The prompts' k / v [B, N, Hk, dh] into empty ring caches, in place."""
+    _req_here(k, v, k_cache, v_cache, lengths)
+    (B, N, Hk, dh), _ = _heads(k, 'window_cache_fill k')
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError('window_cache_fill: k and v must match')
+    C = _check_cache('window_cache_fill', k_cache, v_cache, B, Hk, dh, k.dtype, lengths)
+    k, v = _aligned_heads(k), _aligned_heads(v)
+    sk, sv = k.stride(), v.stride()
+    check(lib().vitk_window_cache_fill(_dt(k), B, N, Hk, dh, k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2],
+                                       _ptr(lengths), k_cache.data_ptr(), v_cache.data_ptr(), C, int(sinks), _stream()),
+          'vitk_window_cache_fill')
