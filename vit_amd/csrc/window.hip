@@ -34,24 +34,51 @@ template <typename T> __device__ __forceinline__ void acc_frag(Frag<T>& f, const
 #pragma unroll
     for (int e = 0; e < 8; ++e) frag_set_f(f, e, a[8 * s + e]);
 }
-// the A fragment that goes with it: columns col0 + (l & 31) of a row-major LDS image, rows row0 + the order above.
+// LDS image of a tile: rows of CPR 16-byte chunks without padding (what the asynchronous loads can write: 64 consecutive
+// chunks an instruction); chunk c of row r sits at place c ^ swz(r), so that the rows that one read touches fall on
+// different banks.
+template <typename T, int DP> struct WCfg {
+    static constexpr int EPC = 16 / sizeof(T);          // elements of a 16-byte chunk
+    static constexpr int CPR = DP / EPC;                // chunks of a row
+    static constexpr int LD = DP + EPC;                 // row stride of the results' image (put_rows)
+    static __device__ __forceinline__ int swz(int r) { return CPR % 8 == 0 ? r & 7 : (r >> 1) & 3; }
+};
+// the A fragment that goes with acc_frag: columns col0 + (l & 31) of an image, rows row0 + the order above (row0 % 16 == 0).
 // bf16: transpose reads -- lane 4 q + p of 16 supplies row q, columns 4 p .. 4 p + 3, and receives column l & 15 of the 4
 // rows; needs every lane of the wave.
-__device__ __forceinline__ void col_frag32(Frag<__bf16>& f, const __bf16* img, int ld, int row0, int col0, int lane) {
-    const int i = lane & 15, q = i >> 2, p = i & 3;
-    const __bf16* a = img + (row0 + 4 * (lane >> 5) + q) * ld + col0 + 16 * ((lane >> 4) & 1) + 4 * p;
+template <int DP> __device__ __forceinline__ void col_frag32(Frag<__bf16>& f, const __bf16* img, int row0, int col0, int lane) {
+    using C = WCfg<__bf16, DP>;
+    const int i = lane & 15, q = i >> 2, p = i & 3, r = 4 * (lane >> 5) + q;
+    const int c = (col0 / 8 + 2 * ((lane >> 4) & 1) + (p >> 1)) ^ C::swz(r);
+    const __bf16* a = img + (row0 + r) * DP + 8 * c + 4 * (p & 1);       // rows 8 further on have the same swz
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)a);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(a + 8 * ld));
-    const s16x8 r = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    f.v = __builtin_bit_cast(bf16x8, r);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(a + 8 * DP));
+    const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    f.v = __builtin_bit_cast(bf16x8, v);
 }
-__device__ __forceinline__ void col_frag32(Frag<float>& f, const float* img, int ld, int row0, int col0, int lane) {
-    const float* a = img + (row0 + 4 * (lane >> 5)) * ld + col0 + (lane & 31);
+template <int DP> __device__ __forceinline__ void col_frag32(Frag<float>& f, const float* img, int row0, int col0, int lane) {
+    using C = WCfg<float, DP>;
+    const int cc = lane & 31;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = a[(8 * (e >> 2) + (e & 3)) * ld];
+    for (int e = 0; e < 8; ++e) {
+        const int r = 4 * (lane >> 5) + (e & 3);
+        f.v[e] = img[(row0 + 8 * (e >> 2) + r) * DP + 4 * ((col0 / 4 + cc / 4) ^ C::swz(r)) + (cc & 3)];
+    }
 }
-template <typename T, int LD> __device__ __forceinline__ void row_frag32(Frag<T>& f, const T* img, int row0, int kk, int lane) {
-    frag_load(f, img + (row0 + (lane & 31)) * LD + 16 * kk + 8 * (lane >> 5));
+// row row0 + (l & 31), elements 16 kk + 8 (l >> 5) + e (row0 % 32 == 0)
+template <int DP> __device__ __forceinline__ void row_frag32(Frag<__bf16>& f, const __bf16* img, int row0, int kk, int lane) {
+    const int r = lane & 31;
+    frag_load(f, img + (row0 + r) * DP + 8 * ((2 * kk + (lane >> 5)) ^ WCfg<__bf16, DP>::swz(r)));
+}
+template <int DP> __device__ __forceinline__ void row_frag32(Frag<float>& f, const float* img, int row0, int kk, int lane) {
+    const int r = lane & 31, s = WCfg<float, DP>::swz(r), c = 4 * kk + 2 * (lane >> 5);
+    const float* a = img + (row0 + r) * DP;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(a + 4 * (c ^ s)), y = *reinterpret_cast<const f32x4*>(a + 4 * ((c + 1) ^ s));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f.v[e] = x[e];
+        f.v[4 + e] = y[e];
+    }
 }
 
 struct View {                     // element (b, n, h, d) at b*sb + n*sn + h*sh + d
@@ -83,35 +110,60 @@ __device__ __forceinline__ long xcd_order(long total) {
     return (blockIdx.x >> 3) < per && id < total ? id : -1;
 }
 
-template <typename T, int DP> struct WCfg {
-    static constexpr int EPC = 16 / sizeof(T);          // elements of a 16-byte chunk
-    static constexpr int CPR = DP / EPC;                // chunks of a staged row
-    static constexpr int LD = DP + EPC;                 // LDS row stride: 16 bytes of padding spread the rows over the banks
-};
+typedef __attribute__((address_space(3))) void* lds_ptr;
 
-// Rows [row0, row0 + ROWS) of a strided matrix through registers into LDS; rows outside [0, hi) and columns >= dh are zero.
+// BYTES a lane from a buffer (voff: the lane's byte offset; past the end reads as 0) to dst + BYTES * lane in LDS, without waiting
+template <int BYTES> __device__ __forceinline__ void load_to_lds(const void* base, unsigned bytes, unsigned voff, void* dst) {
+#if defined(__HIP_DEVICE_COMPILE__)       // the host pass does not know this size of the builtin
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+    if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(uintptr_t)dst, 16, voff, 0, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(uintptr_t)dst, 4, voff, 0, 0, 0);
+#endif
+}
+
+// Rows [row0, row0 + ROWS) of a strided matrix into an image, asynchronously and without passing through registers; rows outside
+// [0, hi) and columns >= dh are zero.  The bounds are the buffer descriptor's (what lies outside reads as zero), and the
+// descriptor is moved to every tile's first row, so offsets in it stay small however long the sequence is.  The data is
+// there after the next tile_ready().
 template <typename T, int DP, int ROWS, int NT> struct Stager {
     using C = WCfg<T, DP>;
     static constexpr int CH = ROWS * C::CPR / NT;
     static_assert(CH * NT == ROWS * C::CPR, "a tile is a whole number of chunks a thread");
-    u32x4 r[CH];
-    __device__ __forceinline__ void load(const T* g, long sn, int row0, int hi, int dh) {
+    unsigned off[CH];
+    __device__ __forceinline__ void init(long sn, int dh) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int idx = threadIdx.x + c * NT;
-            const int row = row0 + idx / C::CPR, d = (idx % C::CPR) * C::EPC;
-            r[c] = u32x4{0, 0, 0, 0};
-            if (row < hi && d < dh) r[c] = *reinterpret_cast<const u32x4*>(g + (long)row * sn + d);
+            const int row = idx / C::CPR, d = ((idx % C::CPR) ^ C::swz(row)) * C::EPC;
+            off[c] = d < dh ? (unsigned)(row * (int)sn + d) * (unsigned)sizeof(T) : 0x80000000u;
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void load(const T* g, long sn, int row0, int hi, int dh, T* lds, int wave) const {
+        const int n = min(hi - row0, ROWS);
+        const unsigned bytes = n > 0 ? (unsigned)((n - 1) * (int)sn + dh) * (unsigned)sizeof(T) : 0u;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int idx = threadIdx.x + c * NT;
-            *reinterpret_cast<u32x4*>(lds + (idx / C::CPR) * C::LD + (idx % C::CPR) * C::EPC) = r[c];
-        }
+        for (int c = 0; c < CH; ++c) load_to_lds<16>(g + (long)row0 * sn, bytes, off[c], lds + (c * NT + 64 * wave) * C::EPC);
     }
 };
+__device__ __forceinline__ void tile_ready() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's asynchronous loads; the barrier: everyone's
+    __syncthreads();
+}
+// ROWS floats of the rows' statistics, the same way (by one wave)
+template <int ROWS> __device__ __forceinline__ void load_stat(const float* g, int row0, int hi, float* lds, int lane) {
+    const int n = min(hi - row0, ROWS);
+    if (ROWS == 64 || lane < ROWS) load_to_lds<4>(g + row0, n > 0 ? 4u * n : 0u, 4u * lane, lds);
+}
+
+// the other half-wave's value joined in: every lane gets f of lanes l and l ^ 32
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
 
 // this wave's 32 rows of a strided matrix as fragments (rows outside [0, hi) are zero)
 template <typename T, int DP>
@@ -195,14 +247,14 @@ __device__ __forceinline__ int tile_kind(const WindowParams& p, int i, int j0, i
 
 // ---------------------------------------------------------------------------------------------------------- forward
 template <typename T, int DP, int NW, int BK>
-__global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams p) {
+__global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * C::LD;
+    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (K tile, V tile)
     const long id = xcd_order(p.total);
     if (id < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // order of the work: the group's heads, then query tiles, then (sequence, key head); causal: long rows first
     const int g = (int)(id % p.G);
     const long r1 = id / p.G;
@@ -224,25 +276,26 @@ __global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams 
     for (int t = 0; t < ND; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
-    float m = -INFINITY, l = 0.f;                        // running maximum (log2 domain) and this half-wave's part of the sum
+    float m = -INFINITY;                                 // running maximum, log2 domain
+    float ls[4] = {0.f, 0.f, 0.f, 0.f};                  // the sum of this lane's keys, in four chains
 
     Stager<T, DP, BK, NT> sk, sv;
+    sk.init(p.k.sn, p.dh);
+    sv.init(p.v.sn, p.dh);
     if (kt.n > 0) {
         const int j0 = BK * key_tile(kt, 0);
-        sk.load(K, p.k.sn, j0, len, p.dh);
-        sv.load(V, p.v.sn, j0, len, p.dh);
-        sk.store(lds);
-        sv.store(lds + TILE);
+        sk.load(K, p.k.sn, j0, len, p.dh, lds, wave);
+        sv.load(V, p.v.sn, j0, len, p.dh, lds + TILE, wave);
     }
     for (int it = 0; it < kt.n; ++it) {
         const T* Ks = lds + (it & 1) * 2 * TILE;
         const T* Vs = Ks + TILE;
-        __syncthreads();                                 // this tile is staged; the other buffer's readers are done
-        const bool more = it + 1 < kt.n;
-        if (more) {
+        tile_ready();                                    // and the other buffer's readers are done
+        if (it + 1 < kt.n) {
             const int j1 = BK * key_tile(kt, it + 1);
-            sk.load(K, p.k.sn, j1, len, p.dh);
-            sv.load(V, p.v.sn, j1, len, p.dh);
+            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
+            sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
+            sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
         }
         const int j0 = BK * key_tile(kt, it);
         const int kind = tile_kind(p, iw, j0, BK, len);  // the same for the whole wave
@@ -256,7 +309,7 @@ __global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams 
 #pragma unroll
                 for (int kk = 0; kk < KD; ++kk) {
                     Frag<T> a;
-                    row_frag32<T, C::LD>(a, Ks, 32 * u, kk, lane);
+                    row_frag32<DP>(a, Ks, 32 * u, kk, lane);
                     s[u] = mma32(a, qf[kk], s[u]);
                 }
             }
@@ -274,13 +327,14 @@ __global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams 
             for (int u = 0; u < NS; ++u)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * p.sc2;
+            mt = half_max(mt) * p.sc2;
             // the reference point only has to keep exp2 in range: it moves when a row's maximum has grown by 2^8
             if (__any(mt > m + 8.f)) {
                 const float mn = fmaxf(m, mt);
                 const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
-                l *= al;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ls[e] *= al;
 #pragma unroll
                 for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -307,7 +361,7 @@ __global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     s[u][e] = __builtin_amdgcn_exp2f(s[u][e]);
-                    l += s[u][e];
+                    ls[e & 3] += s[u][e];
                 }
 #pragma unroll
             for (int u = 0; u < NS; ++u)
@@ -318,18 +372,13 @@ __global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams 
 #pragma unroll
                     for (int t = 0; t < ND; ++t) {
                         Frag<T> a;
-                        col_frag32(a, Vs, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                        col_frag32<DP>(a, Vs, 32 * u + 16 * ks, 32 * t, lane);
                         o[t] = mma32(a, pf, o[t]);
                     }
                 }
         }
-        if (more) {
-            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
-            sk.store(nx);
-            sv.store(nx + TILE);
-        }
     }
-    l += __shfl_xor(l, 32, 64);
+    const float l = half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
     const bool none = i >= len || (m == -INFINITY && l == 0.f);      // nothing visible (a NaN sum stays a NaN)
     if (p.lse && lane < 32 && i < p.N) p.lse[((long)b * p.Hq + h) * p.N + i] = none ? INFINITY : m + __log2f(l);
     __syncthreads();
@@ -338,15 +387,15 @@ __global__ __launch_bounds__(64 * NW) void window_fwd_kernel(const WindowParams 
 }
 
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
-template <typename T, int DP, int NW, int BK>
-__global__ __launch_bounds__(64 * NW) void window_dq_kernel(const WindowParams p) {
+template <typename T, int DP, int NW, int BK, int WPE>
+__global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * C::LD;
+    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);
     const long id = xcd_order(p.total);
     if (id < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = (int)(id % p.G);
     const long r1 = id / p.G;
     const int tq = (int)(r1 % p.tiles), bh = (int)(r1 / p.tiles);
@@ -372,7 +421,7 @@ __global__ __launch_bounds__(64 * NW) void window_dq_kernel(const WindowParams p
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta += frag_get_f(of[0], e) * frag_get_f(df[kk], e);
         }
-        delta += __shfl_xor(delta, 32, 64);
+        delta = half_sum(delta);
         const long at = ((long)b * p.Hq + h) * p.N + i;
         if (i < len) lse = p.lse[at];
         if (lane < 32 && i < p.N) p.delta[at] = delta;
@@ -386,22 +435,22 @@ __global__ __launch_bounds__(64 * NW) void window_dq_kernel(const WindowParams p
         for (int e = 0; e < 16; ++e) dq[t][e] = 0.f;
 
     Stager<T, DP, BK, NT> sk, sv;
+    sk.init(p.k.sn, p.dh);
+    sv.init(p.v.sn, p.dh);
     if (kt.n > 0) {
         const int j0 = BK * key_tile(kt, 0);
-        sk.load(K, p.k.sn, j0, len, p.dh);
-        sv.load(V, p.v.sn, j0, len, p.dh);
-        sk.store(lds);
-        sv.store(lds + TILE);
+        sk.load(K, p.k.sn, j0, len, p.dh, lds, wave);
+        sv.load(V, p.v.sn, j0, len, p.dh, lds + TILE, wave);
     }
     for (int it = 0; it < kt.n; ++it) {
         const T* Ks = lds + (it & 1) * 2 * TILE;
         const T* Vs = Ks + TILE;
-        __syncthreads();
-        const bool more = it + 1 < kt.n;
-        if (more) {
+        tile_ready();
+        if (it + 1 < kt.n) {
             const int j1 = BK * key_tile(kt, it + 1);
-            sk.load(K, p.k.sn, j1, len, p.dh);
-            sv.load(V, p.v.sn, j1, len, p.dh);
+            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
+            sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
+            sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
         }
         const int j0 = BK * key_tile(kt, it);
         const int kind = tile_kind(p, iw, j0, BK, len);
@@ -414,9 +463,9 @@ __global__ __launch_bounds__(64 * NW) void window_dq_kernel(const WindowParams p
 #pragma unroll
                 for (int kk = 0; kk < KD; ++kk) {
                     Frag<T> a;
-                    row_frag32<T, C::LD>(a, Ks, 32 * u, kk, lane);
+                    row_frag32<DP>(a, Ks, 32 * u, kk, lane);
                     s = mma32(a, qf[kk], s);
-                    row_frag32<T, C::LD>(a, Vs, 32 * u, kk, lane);
+                    row_frag32<DP>(a, Vs, 32 * u, kk, lane);
                     dp = mma32(a, df[kk], dp);
                 }
 #pragma unroll
@@ -436,16 +485,11 @@ __global__ __launch_bounds__(64 * NW) void window_dq_kernel(const WindowParams p
 #pragma unroll
                     for (int t = 0; t < ND; ++t) {
                         Frag<T> a;
-                        col_frag32(a, Ks, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                        col_frag32<DP>(a, Ks, 32 * u + 16 * ks, 32 * t, lane);
                         dq[t] = mma32(a, sf, dq[t]);
                     }
                 }
             }
-        }
-        if (more) {
-            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
-            sk.store(nx);
-            sv.store(nx + TILE);
         }
     }
     __syncthreads();
@@ -457,16 +501,16 @@ __global__ __launch_bounds__(64 * NW) void window_dq_kernel(const WindowParams p
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
 // every head of the group.  SINK: one wave, the 32 keys of a sinks' tile and a share of ALL the query tiles, fp32 partial
 // sums out (window_sink_sum_kernel adds the shares in order).
-template <typename T, int DP, int NW, int BQ, bool SINK>
-__global__ __launch_bounds__(64 * NW) void window_dkv_kernel(const WindowParams p) {
+template <typename T, int DP, int NW, int BQ, bool SINK, int WPE>
+__global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, NS = BQ / 32, KD = DP / 16, ND = DP / 32, TILE = BQ * C::LD;
+    constexpr int NT = 64 * NW, NS = BQ / 32, KD = DP / 16, ND = DP / 32, TILE = BQ * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (Q tile, dO tile), then of BQ (lse, D) each
     float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
     const long id = xcd_order(p.total);
     if (id < 0) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int chunk = 0;
     long r1 = id;
     if (SINK) {
@@ -511,38 +555,25 @@ __global__ __launch_bounds__(64 * NW) void window_dkv_kernel(const WindowParams 
         for (int e = 0; e < 16; ++e) dk[t][e] = dv[t][e] = 0.f;
 
     Stager<T, DP, BQ, NT> sq, sd;
-    float st0 = INFINITY, st1 = 0.f;                     // thread's (lse, D): thread t < BQ holds row t
+    sq.init(p.q.sn, p.dh);
+    sd.init(p.dout.sn, p.dh);
+    // rows past the end come as zeros, statistics too: their p is 1 there, and meets zeros of dO, D and Q
     auto fetch = [&](int it) {
         const int h = hk * p.G + it / nt, i0 = BQ * (ta + it % nt);
-        sq.load(static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i0, len, p.dh);
-        sd.load(static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i0, len, p.dh);
-        st0 = INFINITY;
-        st1 = 0.f;
-        const int i = i0 + (int)threadIdx.x;
-        if ((int)threadIdx.x < BQ && i < len) {
-            const long at = ((long)b * p.Hq + h) * p.N + i;
-            st0 = p.lse[at];
-            st1 = p.delta[at];
-        }
-    };
-    auto put = [&](int it) {
         T* nx = lds + (it & 1) * 2 * TILE;
-        sq.store(nx);
-        sd.store(nx + TILE);
-        if ((int)threadIdx.x < BQ) {
-            stat[(it & 1) * 2 * BQ + threadIdx.x] = st0;
-            stat[(it & 1) * 2 * BQ + BQ + threadIdx.x] = st1;
-        }
+        sq.load(static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i0, len, p.dh, nx, wave);
+        sd.load(static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i0, len, p.dh, nx + TILE, wave);
+        float* ns = stat + (it & 1) * 2 * BQ;
+        const long at = ((long)b * p.Hq + h) * p.N;
+        if (wave == 0) load_stat<BQ>(p.lse + at, i0, len, ns, lane);
+        if (wave == NW - 1) load_stat<BQ>(p.delta + at, i0, len, ns + BQ, lane);
     };
-    if (it0 < it1) {
-        fetch(it0);
-        put(it0);
-    }
+    if (it0 < it1) fetch(it0);
     for (int it = it0; it < it1; ++it) {
         const T* Qs = lds + (it & 1) * 2 * TILE;
         const T* Ds = Qs + TILE;
         const float* ls = stat + (it & 1) * 2 * BQ;
-        __syncthreads();
+        tile_ready();
         if (it + 1 < it1) fetch(it + 1);
         const int i0 = BQ * (ta + it % nt);
 #pragma unroll
@@ -556,9 +587,9 @@ __global__ __launch_bounds__(64 * NW) void window_dkv_kernel(const WindowParams 
 #pragma unroll
             for (int kk = 0; kk < KD; ++kk) {
                 Frag<T> a;
-                row_frag32<T, C::LD>(a, Qs, 32 * u, kk, lane);
+                row_frag32<DP>(a, Qs, 32 * u, kk, lane);
                 s = mma32(a, kf[kk], s);
-                row_frag32<T, C::LD>(a, Ds, 32 * u, kk, lane);
+                row_frag32<DP>(a, Ds, 32 * u, kk, lane);
                 dp = mma32(a, vf[kk], dp);
             }
 #pragma unroll
@@ -586,14 +617,13 @@ __global__ __launch_bounds__(64 * NW) void window_dkv_kernel(const WindowParams 
 #pragma unroll
                 for (int t = 0; t < ND; ++t) {
                     Frag<T> a;
-                    col_frag32(a, Ds, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                    col_frag32<DP>(a, Ds, 32 * u + 16 * ks, 32 * t, lane);
                     dv[t] = mma32(a, pf, dv[t]);
-                    col_frag32(a, Qs, C::LD, 32 * u + 16 * ks, 32 * t, lane);
+                    col_frag32<DP>(a, Qs, 32 * u + 16 * ks, 32 * t, lane);
                     dk[t] = mma32(a, sf, dk[t]);
                 }
             }
         }
-        if (it + 1 < it1) put(it + 1);
     }
     if (SINK) {
         float* o = p.part + id * 2 * DP * 32;
@@ -614,28 +644,29 @@ __global__ __launch_bounds__(64 * NW) void window_dkv_kernel(const WindowParams 
     put_rows<T, DP>(dv, 1.f, j >= len, mine, static_cast<T*>(p.dv) + at, ldg, jw, p.N, p.dh, lane);
 }
 
-// rows of the sinks' tiles: the shares' sum, rounded once.  One workgroup a (sequence, key head, tile).
+// rows of the sinks' tiles: the shares' sum in order, rounded once.  A workgroup takes 8 head elements of one (sequence, key
+// head, tile), dk or dv: 32 keys x 8 elements, one a thread, so its reads are whole rows of the partial sums.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void window_sink_sum_kernel(const WindowParams p) {
-    __shared__ float t[32][DP + 1];
-    const int tk = blockIdx.x % p.tiles, bh = blockIdx.x / p.tiles;
+    __shared__ float t[32][9];
+    const int d0 = 8 * (blockIdx.x % (DP / 8)), which = blockIdx.x / (DP / 8) % 2;
+    const long set = blockIdx.x / (DP / 8) / 2;
+    const int tk = (int)(set % p.tiles), bh = (int)(set / p.tiles);
     const int b = bh / p.Hk, hk = bh % p.Hk;
-    const float* part = p.part + (long)blockIdx.x * p.chunks * 2 * DP * 32;
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
-        T* out = static_cast<T*>(which ? p.dv : p.dk);
-        for (int e = threadIdx.x; e < DP * 32; e += 256) {
-            float s = 0.f;
-            for (int c = 0; c < p.chunks; ++c) s += part[((long)c * 2 + which) * DP * 32 + e];
-            t[e & 31][e >> 5] = which ? s : s * p.scale;
-        }
-        __syncthreads();
-        for (int e = threadIdx.x; e < DP * 32; e += 256) {
-            const int r = e / DP, d = e % DP, j = 32 * tk + r;
-            if (j < p.N && d < p.dh) out[(((long)b * p.N + j) * p.Hk + hk) * p.dh + d] = (T)t[r][d];
-        }
-        __syncthreads();
-    }
+    if (d0 >= p.dh) return;
+    const float* part = p.part + (set * p.chunks * 2 + which) * DP * 32 + d0 * 32 + threadIdx.x;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    int c = 0;
+    for (; c + 8 <= p.chunks; c += 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += part[(long)(c + e) * 2 * DP * 32];
+    for (; c < p.chunks; ++c) s[0] += part[(long)c * 2 * DP * 32];
+    const float sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    t[threadIdx.x & 31][threadIdx.x >> 5] = which ? sum : sum * p.scale;
+    __syncthreads();
+    const int r = threadIdx.x >> 3, d = d0 + (threadIdx.x & 7), j = 32 * tk + r;
+    T* out = static_cast<T*>(which ? p.dv : p.dk);
+    if (j < p.N) out[(((long)b * p.N + j) * p.Hk + hk) * p.dh + d] = (T)t[r][threadIdx.x & 7];
 }
 
 }  // namespace vitk
@@ -688,6 +719,7 @@ int check_view(const char* what, const char* name, const View& v, int dtype) {
     const int per = dtype == VITK_F32 ? 4 : 8;
     VITK_CHECK_ARG(v.p && (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.sb % per == 0 && v.sn % per == 0 && v.sh % per == 0,
                    "%s: %s must be 16-byte aligned, its strides too", what, name);
+    VITK_CHECK_ARG(v.sn >= 0 && v.sn < (1L << 23), "%s: the tokens of %s are too far apart", what, name);    // 64 rows under 2 GiB
     return VITK_OK;
 }
 void fill_params(WindowParams& p, int B, int N, int Hq, int Hk, int dh, int w, int S, int causal, float scale, const int* lengths) {
@@ -705,28 +737,29 @@ template <typename T, int DP, int NW> int run_fwd(WindowParams p, hipStream_t st
     constexpr int BK = sizeof(T) == 2 ? 64 : 32;
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     p.total = (long)p.B * p.Hq * p.tiles;
-    const size_t tiles = 4 * BK * WCfg<T, DP>::LD * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
+    const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK>), lds);
     hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
     return VITK_OK;
 }
 template <typename T, int DP, int NW> void run_dq(WindowParams p, hipStream_t st) {
-    constexpr int BK = sizeof(T) == 2 ? 64 : 32;
+    constexpr int BK = sizeof(T) == 2 ? 64 : 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;   // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     p.total = (long)p.B * p.Hq * p.tiles;
-    const size_t tiles = 4 * BK * WCfg<T, DP>::LD * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
+    const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK>), lds);
-    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK, WPE>), lds);
+    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK, WPE>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
 }
 template <typename T, int DP, int NW, int BQ, bool SINK> void run_dkv(WindowParams p, int tiles, hipStream_t st) {
+    constexpr int WPE = sizeof(T) == 4 && DP >= 96 ? 1 : 2;
     p.tiles = tiles;
     p.total = (long)p.B * p.Hk * tiles * (SINK ? p.chunks : 1);
-    const size_t tl = 4 * BQ * WCfg<T, DP>::LD * sizeof(T) + 4 * BQ * sizeof(float), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
+    const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tl > rows ? tl : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK>), lds);
-    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, WPE>), lds);
+    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, WPE>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
 }
 template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
     constexpr int BQ = sizeof(T) == 2 ? 64 : 32;
@@ -740,7 +773,8 @@ template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void*
         s.per_chunk = pl.per_chunk;
         run_dkv<T, DP, 1, SINK_BQ, true>(s, pl.sink_keys / 32, st);
         s.tiles = pl.sink_keys / 32;
-        hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles)), dim3(256), 0, st, s);
+        hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles * 2 * (DP / 8))), dim3(256),
+                           0, st, s);
     }
     p.key0 = pl.sink_keys;
     const int rest = p.N - pl.sink_keys;
