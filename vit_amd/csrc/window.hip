@@ -35,13 +35,18 @@ template <typename T> __device__ __forceinline__ void acc_frag(Frag<T>& f, const
     for (int e = 0; e < 8; ++e) frag_set_f(f, e, a[8 * s + e]);
 }
 // LDS image of a tile: rows of CPR 16-byte chunks without padding (what the asynchronous loads can write: 64 consecutive
-// chunks an instruction); chunk c of row r sits at place c ^ swz(r), so that the rows that one read touches fall on
-// different banks.
+// chunks an instruction); chunk c of row r sits at place c ^ swz(r).  The 64 banks hold 16 chunks.  A row fragment reads
+// one chunk of each row: over 16 rows swz (with the row's own offset where a row is shorter than the banks) takes every
+// value.  A transpose read takes 4 chunks of each of 4 rows: its low two bits stay among those 4, its upper bits (or the
+// row's offset) send the 4 rows to different quarters of the banks.  With swz = r & 7, two thirds of the LDS time at 128
+// wide heads were conflicts.
 template <typename T, int DP> struct WCfg {
     static constexpr int EPC = 16 / sizeof(T);          // elements of a 16-byte chunk
     static constexpr int CPR = DP / EPC;                // chunks of a row
     static constexpr int LD = DP + EPC;                 // row stride of the results' image (put_rows)
-    static __device__ __forceinline__ int swz(int r) { return CPR % 8 == 0 ? r & 7 : (r >> 1) & 3; }
+    static __device__ __forceinline__ int swz(int r) {
+        return CPR % 16 == 0 ? ((r & 3) << 2) | ((r >> 2) & 3) : (CPR % 8 == 0 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3);
+    }
 };
 // the A fragment that goes with acc_frag: columns col0 + (l & 31) of an image, rows row0 + the order above (row0 % 16 == 0).
 // bf16: transpose reads -- lane 4 q + p of 16 supplies row q, columns 4 p .. 4 p + 3, and receives column l & 15 of the 4
@@ -50,9 +55,10 @@ template <int DP> __device__ __forceinline__ void col_frag32(Frag<__bf16>& f, co
     using C = WCfg<__bf16, DP>;
     const int i = lane & 15, q = i >> 2, p = i & 3, r = 4 * (lane >> 5) + q;
     const int c = (col0 / 8 + 2 * ((lane >> 4) & 1) + (p >> 1)) ^ C::swz(r);
-    const __bf16* a = img + (row0 + r) * DP + 8 * c + 4 * (p & 1);       // rows 8 further on have the same swz
+    const __bf16* a = img + (row0 + r) * DP + 8 * c + 4 * (p & 1);
+    const __bf16* b = img + (row0 + r + 8) * DP + 8 * (c ^ 2) + 4 * (p & 1);             // swz(r + 8) = swz(r) ^ 2 here (r < 8)
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)a);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)(a + 8 * DP));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)b);
     const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     f.v = __builtin_bit_cast(bf16x8, v);
 }
@@ -61,8 +67,8 @@ template <int DP> __device__ __forceinline__ void col_frag32(Frag<float>& f, con
     const int cc = lane & 31;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int r = 4 * (lane >> 5) + (e & 3);
-        f.v[e] = img[(row0 + 8 * (e >> 2) + r) * DP + 4 * ((col0 / 4 + cc / 4) ^ C::swz(r)) + (cc & 3)];
+        const int r = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        f.v[e] = img[(row0 + r) * DP + 4 * ((col0 / 4 + cc / 4) ^ C::swz(r)) + (cc & 3)];
     }
 }
 // row row0 + (l & 31), elements 16 kk + 8 (l >> 5) + e (row0 % 32 == 0)
