@@ -104,28 +104,41 @@ struct WindowParams {
     int tiles;                    // query tiles / key tiles of a sequence
     int key0;                     // keys' kernel: first key (the sinks before it have their own launch)
     int chunks, per_chunk;        // sinks' launch: query tiles are dealt to `chunks` workgroups
-    long total;                   // workgroups that have work (the grid is rounded up to whole rounds of the 8 XCDs)
+    int total;                    // workgroups that have work (the grid is rounded up to whole rounds of the 8 XCDs)
     float scale, sc2;             // sc2 = scale * log2(e)
 };
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Workgroups are dealt to the 8 XCDs in turn; neighbours in the work (same keys, other head of the group; next query tile)
 // should share an L2, so XCD x takes the x-th eighth of the work in order.
-__device__ __forceinline__ long xcd_order(long total) {
-    const long per = (total + 7) / 8;
-    const long id = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    return (blockIdx.x >> 3) < per && id < total ? id : -1;
+__device__ __forceinline__ int xcd_order(int total) {
+    const int per = (total + 7) / 8;
+    const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    return id < total ? id : -1;
 }
 
-typedef __attribute__((address_space(3))) void* lds_ptr;
-
-// BYTES a lane from a buffer (voff: the lane's byte offset; past the end reads as 0) to dst + BYTES * lane in LDS, without waiting
+// BYTES a lane from a buffer (voff: the lane's byte offset; past the end reads as 0) to dst + BYTES * lane in LDS, without waiting:
+// tile_ready() does.  In assembly (there is no result register that could be reused too early), because the compiler takes
+// the transpose reads of the present tile for readers of whatever the builtin is writing, and waits for the next tile in
+// front of them.  m0 is the LDS address; it wants one wait state before its use, and nothing else in these kernels uses it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int BYTES> __device__ __forceinline__ void load_to_lds(const void* base, unsigned bytes, unsigned voff, void* dst) {
-#if defined(__HIP_DEVICE_COMPILE__)       // the host pass does not know this size of the builtin
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
-    if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(uintptr_t)dst, 16, voff, 0, 0, 0);
-    else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(uintptr_t)dst, 4, voff, 0, 0, 0);
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef __attribute__((ext_vector_type(4))) unsigned rsrc_t;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(base);
+    const rsrc_t rs = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu),
+                       (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>(dst));
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff), "s"(rs) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(voff), "s"(rs) : "memory", "m0");
 #endif
 }
+#pragma clang diagnostic pop
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }     // vmcnt(0), in a form the compiler counts
 
 // Rows [row0, row0 + ROWS) of a strided matrix into an image, asynchronously and without passing through registers; rows outside
 // [0, hi) and columns >= dh are zero.  The bounds are the buffer descriptor's (what lies outside reads as zero), and the
@@ -133,8 +146,8 @@ template <int BYTES> __device__ __forceinline__ void load_to_lds(const void* bas
 // there after the next tile_ready().
 template <typename T, int DP, int ROWS, int NT> struct Stager {
     using C = WCfg<T, DP>;
-    static constexpr int CH = ROWS * C::CPR / NT;
-    static_assert(CH * NT == ROWS * C::CPR, "a tile is a whole number of chunks a thread");
+    static constexpr int LOADS = ROWS * C::CPR / 64, CH = (LOADS + NT / 64 - 1) / (NT / 64);    // of the workgroup, of a wave
+    static_assert(LOADS * 64 == ROWS * C::CPR, "a tile is a whole number of loads");
     unsigned off[CH];
     __device__ __forceinline__ void init(long sn, int dh) {
 #pragma unroll
@@ -148,11 +161,14 @@ template <typename T, int DP, int ROWS, int NT> struct Stager {
         const int n = min(hi - row0, ROWS);
         const unsigned bytes = n > 0 ? (unsigned)((n - 1) * (int)sn + dh) * (unsigned)sizeof(T) : 0u;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) load_to_lds<16>(g + (long)row0 * sn, bytes, off[c], lds + (c * NT + 64 * wave) * C::EPC);
+        for (int c = 0; c < CH; ++c)
+            if (LOADS % (NT / 64) == 0 || c * (NT / 64) + wave < LOADS)
+                load_to_lds<16>(g + (long)row0 * sn, bytes, off[c], lds + (c * NT + 64 * wave) * C::EPC);
     }
 };
 __device__ __forceinline__ void tile_ready() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // this wave's asynchronous loads; the barrier: everyone's
+    asm volatile("" ::: "memory");
+    loads_done();                                        // this wave's asynchronous loads; the barrier: everyone's
     __syncthreads();
 }
 // ROWS floats of the rows' statistics, the same way (by one wave)
@@ -240,10 +256,10 @@ __device__ __forceinline__ RowRange row_range(const WindowParams& p, int i, int 
     r.s = min(p.S, e + 1);
     return r;
 }
-// for a wave's queries [i, i + 32) and keys [j0, j0 + BK): 0 nothing visible, 1 some, 2 all
-__device__ __forceinline__ int tile_kind(const WindowParams& p, int i, int j0, int BK, int len) {
+// for a wave's queries [i, i + BQ) and keys [j0, j0 + BK): 0 nothing visible, 1 some, 2 all
+__device__ __forceinline__ int tile_kind(const WindowParams& p, int i, int BQ, int j0, int BK, int len) {
     if (i >= len) return 0;
-    const int j1 = j0 + BK - 1, i1 = i + 31;
+    const int j1 = j0 + BK - 1, i1 = i + BQ - 1;
     if (p.causal && j0 > i1) return 0;
     const bool in = p.w < 0 || (j1 >= i - p.w && j0 <= i1 + p.w);
     if (!in && j0 >= p.S) return 0;
@@ -258,16 +274,15 @@ __global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowPara
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (K tile, V tile)
-    const long id = xcd_order(p.total);
+    const int id = xcd_order(p.total);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // order of the work: the group's heads, then query tiles, then (sequence, key head); causal: long rows first
-    const int g = (int)(id % p.G);
-    const long r1 = id / p.G;
-    const int tq = (int)(r1 % p.tiles), bh = (int)(r1 / p.tiles);
-    const int b = bh / p.Hk, hk = bh % p.Hk, h = hk * p.G + g;
+    const int r1 = uniform(id / p.G), g = id - r1 * p.G;
+    const int bh = uniform(r1 / p.tiles), tq = r1 - bh * p.tiles;
+    const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk, h = hk * p.G + g;
     const int i0 = 32 * NW * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * wave;
-    const int len = p.lengths ? max(0, min(p.lengths[b], p.N)) : p.N;
+    const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
     const int i = iw + (lane & 31);
 
     const T* K = static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh;
@@ -285,6 +300,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowPara
     float m = -INFINITY;                                 // running maximum, log2 domain
     float ls[4] = {0.f, 0.f, 0.f, 0.f};                  // the sum of this lane's keys, in four chains
 
+    loads_done();                                        // nothing but tiles is in flight in the loop
     Stager<T, DP, BK, NT> sk, sv;
     sk.init(p.k.sn, p.dh);
     sv.init(p.v.sn, p.dh);
@@ -304,7 +320,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowPara
             sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
         }
         const int j0 = BK * key_tile(kt, it);
-        const int kind = tile_kind(p, iw, j0, BK, len);  // the same for the whole wave
+        const int kind = tile_kind(p, iw, 32, j0, BK, len);  // the same for the whole wave
         if (kind) {
             f32x16 s[NS];
             float mt = -INFINITY;
@@ -399,15 +415,14 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);
-    const long id = xcd_order(p.total);
+    const int id = xcd_order(p.total);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = (int)(id % p.G);
-    const long r1 = id / p.G;
-    const int tq = (int)(r1 % p.tiles), bh = (int)(r1 / p.tiles);
-    const int b = bh / p.Hk, hk = bh % p.Hk, h = hk * p.G + g;
+    const int r1 = uniform(id / p.G), g = id - r1 * p.G;
+    const int bh = uniform(r1 / p.tiles), tq = r1 - bh * p.tiles;
+    const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk, h = hk * p.G + g;
     const int i0 = 32 * NW * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * wave;
-    const int len = p.lengths ? max(0, min(p.lengths[b], p.N)) : p.N;
+    const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
     const int i = iw + (lane & 31);
 
     const T* K = static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh;
@@ -440,6 +455,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 #pragma unroll
         for (int e = 0; e < 16; ++e) dq[t][e] = 0.f;
 
+    loads_done();                                        // nothing but tiles is in flight in the loop
     Stager<T, DP, BK, NT> sk, sv;
     sk.init(p.k.sn, p.dh);
     sv.init(p.v.sn, p.dh);
@@ -459,7 +475,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
             sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
         }
         const int j0 = BK * key_tile(kt, it);
-        const int kind = tile_kind(p, iw, j0, BK, len);
+        const int kind = tile_kind(p, iw, 32, j0, BK, len);
         if (kind) {
 #pragma unroll
             for (int u = 0; u < NS; ++u) {
@@ -507,30 +523,32 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
 // every head of the group.  SINK: one wave, the 32 keys of a sinks' tile and a share of ALL the query tiles, fp32 partial
 // sums out (window_sink_sum_kernel adds the shares in order).
-template <typename T, int DP, int NW, int BQ, bool SINK, int WPE>
+template <typename T, int DP, int NW, int BQ, bool SINK, bool VLDS, int WPE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
     constexpr int NT = 64 * NW, NS = BQ / 32, KD = DP / 16, ND = DP / 32, TILE = BQ * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (Q tile, dO tile), then of BQ (lse, D) each
     float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
-    const long id = xcd_order(p.total);
+    const int id = xcd_order(p.total);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int chunk = 0;
-    long r1 = id;
+    int r1 = id;
     if (SINK) {
-        chunk = (int)(id % p.chunks);
-        r1 = id / p.chunks;
+        r1 = uniform(id / p.chunks);
+        chunk = id - r1 * p.chunks;
     }
-    const int tk = (int)(r1 % p.tiles), bh = (int)(r1 / p.tiles);
-    const int b = bh / p.Hk, hk = bh % p.Hk;
+    const int bh = uniform(r1 / p.tiles), tk = r1 - bh * p.tiles;
+    const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk;
     const int j0 = p.key0 + 32 * NW * tk, jw = j0 + 32 * wave, j = jw + (lane & 31);
-    const int len = p.lengths ? max(0, min(p.lengths[b], p.N)) : p.N;
+    const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
 
-    Frag<T> kf[KD], vf[KD];
+    Frag<T> kf[KD], vf[VLDS ? 1 : KD];
+    T* Vs = reinterpret_cast<T*>(stat + 4 * BQ);         // VLDS: the workgroup's V rows stay in LDS
     own_rows<T, DP>(kf, static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh, p.k.sn, j, len, p.dh, lane);
-    own_rows<T, DP>(vf, static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh, p.v.sn, j, len, p.dh, lane);
+    const T* V = static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh;
+    if constexpr (!VLDS) own_rows<T, DP>(vf, V, p.v.sn, j, len, p.dh, lane);
 
     // queries that see key j: i - ilo <= span (unsigned); none for a key past the end
     int ilo = 1 << 30;
@@ -560,12 +578,18 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[t][e] = dv[t][e] = 0.f;
 
+    loads_done();
+    if constexpr (VLDS) {
+        Stager<T, DP, 32 * NW, NT> sv;
+        sv.init(p.v.sn, p.dh);
+        sv.load(V, p.v.sn, j0, len, p.dh, Vs, wave);
+    }
     Stager<T, DP, BQ, NT> sq, sd;
     sq.init(p.q.sn, p.dh);
     sd.init(p.dout.sn, p.dh);
     // rows past the end come as zeros, statistics too: their p is 1 there, and meets zeros of dO, D and Q
     auto fetch = [&](int it) {
-        const int h = hk * p.G + it / nt, i0 = BQ * (ta + it % nt);
+        const int gi = uniform(it / nt), h = hk * p.G + gi, i0 = BQ * (ta + it - gi * nt);
         T* nx = lds + (it & 1) * 2 * TILE;
         sq.load(static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i0, len, p.dh, nx, wave);
         sd.load(static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i0, len, p.dh, nx + TILE, wave);
@@ -574,6 +598,59 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         if (wave == 0) load_stat<BQ>(p.lse + at, i0, len, ns, lane);
         if (wave == NW - 1) load_stat<BQ>(p.delta + at, i0, len, ns + BQ, lane);
     };
+    // 32 queries of a tile: scores and dP, P and dS from them, then dv and dk
+    auto tile = [&](int kind, const T* Qs, const T* Ds, const float* ls, int u, int i0) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KD; ++kk) {
+            Frag<T> a, v;
+            row_frag32<DP>(a, Qs, 32 * u, kk, lane);
+            s = mma32(a, kf[kk], s);
+            row_frag32<DP>(a, Ds, 32 * u, kk, lane);
+            if constexpr (VLDS) {
+                row_frag32<DP>(v, Vs, 32 * wave, kk, lane);
+                dp = mma32(a, v, dp);
+            } else {
+                dp = mma32(a, vf[kk], dp);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = 32 * u + 8 * q + 4 * (lane >> 5);
+            asm volatile("" ::: "memory");               // one quarter's statistics in registers at a time
+            const f32x4 L = *reinterpret_cast<const f32x4*>(ls + row), D = *reinterpret_cast<const f32x4*>(ls + BQ + row);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float pe = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], p.sc2, -L[e]));
+                dp[4 * q + e] = pe * (dp[4 * q + e] - D[e]);
+                s[4 * q + e] = pe;
+            }
+        }
+        if (kind == 1) {                                 // (no second copy of the products: it costs moves of all accumulators)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const bool ok = (unsigned)(i0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) - ilo) <= span;
+                s[e] = ok ? s[e] : 0.f;
+                dp[e] = ok ? dp[e] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            Frag<T> pf, sf;
+            acc_frag(pf, s, ks);
+            acc_frag(sf, dp, ks);
+#pragma unroll
+            for (int t = 0; t < ND; ++t) {
+                Frag<T> a;
+                col_frag32<DP>(a, Ds, 32 * u + 16 * ks, 32 * t, lane);
+                dv[t] = mma32(a, pf, dv[t]);
+                col_frag32<DP>(a, Qs, 32 * u + 16 * ks, 32 * t, lane);
+                dk[t] = mma32(a, sf, dk[t]);
+            }
+        }
+    };
     if (it0 < it1) fetch(it0);
     for (int it = it0; it < it1; ++it) {
         const T* Qs = lds + (it & 1) * 2 * TILE;
@@ -581,58 +658,15 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         const float* ls = stat + (it & 1) * 2 * BQ;
         tile_ready();
         if (it + 1 < it1) fetch(it + 1);
-        const int i0 = BQ * (ta + it % nt);
+        const int i0 = BQ * (ta + it - uniform(it / nt) * nt);
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
-            const int iu = i0 + 32 * u;
-            const int kind = jw < len ? tile_kind(p, iu, jw, 32, len) : 0;
-            if (!kind) continue;
-            f32x16 s, dp;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < KD; ++kk) {
-                Frag<T> a;
-                row_frag32<DP>(a, Qs, 32 * u, kk, lane);
-                s = mma32(a, kf[kk], s);
-                row_frag32<DP>(a, Ds, 32 * u, kk, lane);
-                dp = mma32(a, vf[kk], dp);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = 32 * u + 8 * q + 4 * (lane >> 5);
-                const f32x4 L = *reinterpret_cast<const f32x4*>(ls + row), D = *reinterpret_cast<const f32x4*>(ls + BQ + row);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float pe = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], p.sc2, -L[e]));
-                    float se = pe * (dp[4 * q + e] - D[e]);
-                    if (kind == 1) {
-                        const bool ok = (unsigned)(i0 + row + e - ilo) <= span;
-                        pe = ok ? pe : 0.f;
-                        se = ok ? se : 0.f;
-                    }
-                    s[4 * q + e] = pe;
-                    dp[4 * q + e] = se;
-                }
-            }
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                Frag<T> pf, sf;
-                acc_frag(pf, s, ks);
-                acc_frag(sf, dp, ks);
-#pragma unroll
-                for (int t = 0; t < ND; ++t) {
-                    Frag<T> a;
-                    col_frag32<DP>(a, Ds, 32 * u + 16 * ks, 32 * t, lane);
-                    dv[t] = mma32(a, pf, dv[t]);
-                    col_frag32<DP>(a, Qs, 32 * u + 16 * ks, 32 * t, lane);
-                    dk[t] = mma32(a, sf, dk[t]);
-                }
-            }
+            const int kind = jw < len ? tile_kind(p, i0 + 32 * u, 32, jw, 32, len) : 0;
+            if (kind) tile(kind, Qs, Ds, ls, u, i0);
         }
     }
     if (SINK) {
-        float* o = p.part + id * 2 * DP * 32;
+        float* o = p.part + (long)id * 2 * DP * 32;
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -742,7 +776,7 @@ unsigned xcd_grid(long total) { return (unsigned)((total + 7) / 8 * 8); }
 template <typename T, int DP, int NW> int run_fwd(WindowParams p, hipStream_t st) {
     constexpr int BK = sizeof(T) == 2 ? 64 : 32;
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
-    p.total = (long)p.B * p.Hq * p.tiles;
+    p.total = p.B * p.Hq * p.tiles;
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK>), lds);
@@ -752,23 +786,25 @@ template <typename T, int DP, int NW> int run_fwd(WindowParams p, hipStream_t st
 template <typename T, int DP, int NW> void run_dq(WindowParams p, hipStream_t st) {
     constexpr int BK = sizeof(T) == 2 ? 64 : 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;   // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
-    p.total = (long)p.B * p.Hq * p.tiles;
+    p.total = p.B * p.Hq * p.tiles;
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK, WPE>), lds);
     hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK, WPE>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
 }
 template <typename T, int DP, int NW, int BQ, bool SINK> void run_dkv(WindowParams p, int tiles, hipStream_t st) {
-    constexpr int WPE = sizeof(T) == 4 && DP >= 96 ? 1 : 2;
+    // V rows in LDS where they, K's and both accumulators do not fit the registers of two waves a SIMD
+    constexpr bool VLDS = sizeof(T) == 2 && DP >= 96 && !SINK;
+    constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK ? 1 : 2;
     p.tiles = tiles;
-    p.total = (long)p.B * p.Hk * tiles * (SINK ? p.chunks : 1);
-    const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
+    p.total = p.B * p.Hk * tiles * (SINK ? p.chunks : 1);
+    const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * NW * DP * sizeof(T) : 0), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tl > rows ? tl : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, WPE>), lds);
-    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, WPE>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), lds);
+    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
 }
 template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
-    constexpr int BQ = sizeof(T) == 2 ? 64 : 32;
+    constexpr int BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     p.out = dq;
     if (pl.nwq == 4) run_dq<T, DP, 4>(p, st);
     else run_dq<T, DP, 2>(p, st);
