@@ -104,17 +104,18 @@ struct WindowParams {
     int tiles;                    // query tiles / key tiles of a sequence
     int key0;                     // keys' kernel: first key (the sinks before it have their own launch)
     int chunks, per_chunk;        // sinks' launch: query tiles are dealt to `chunks` workgroups
+    int run;                      // consecutive pieces of work an XCD takes at a time
     int total;                    // workgroups that have work (the grid is rounded up to whole rounds of the 8 XCDs)
     float scale, sc2;             // sc2 = scale * log2(e)
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Workgroups are dealt to the 8 XCDs in turn; neighbours in the work (same keys, other head of the group; next query tile)
-// should share an L2, so XCD x takes the x-th eighth of the work in order.
-__device__ __forceinline__ int xcd_order(int total) {
-    const int per = (total + 7) / 8;
-    const int id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+// Workgroups are dealt to the 8 XCDs in turn.  Neighbours in the work (same keys, other head of the group; next tile) should
+// share an L2, so an XCD takes runs of `run` consecutive pieces of work.
+__device__ __forceinline__ int xcd_order(int total, int run) {
+    const int slot = (int)(blockIdx.x >> 3), r = uniform(slot / run);
+    const int id = (r * 8 + (int)(blockIdx.x & 7)) * run + slot - r * run;
     return id < total ? id : -1;
 }
 
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowPara
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (K tile, V tile)
-    const int id = xcd_order(p.total);
+    const int id = xcd_order(p.total, p.run);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // order of the work: the group's heads, then query tiles, then (sequence, key head); causal: long rows first
@@ -415,7 +416,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);
-    const int id = xcd_order(p.total);
+    const int id = xcd_order(p.total, p.run);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r1 = uniform(id / p.G), g = id - r1 * p.G;
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (Q tile, dO tile), then of BQ (lse, D) each
     float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
-    const int id = xcd_order(p.total);
+    const int id = xcd_order(p.total, p.run);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int chunk = 0;
@@ -771,37 +772,46 @@ void fill_params(WindowParams& p, int B, int N, int Hq, int Hk, int dh, int w, i
     p.scale = scale;
     p.sc2 = scale * 1.4426950408889634f;
 }
-unsigned xcd_grid(long total) { return (unsigned)((total + 7) / 8 * 8); }
+// Sets p.total and p.run; the grid that goes with them.  Pieces of equal work: an eighth of them in a row to each XCD (causal
+// 16384 x 128, groups of 4 heads: 180 us forward, with runs of 64 or 16 pieces 194).  Pieces that differ (sequences of
+// different lengths, causal rows without a window): runs of 16, fewer where there is little work (three sequences of 1001
+// tokens and less, fp32: forward 167 us, with an eighth in a row 219).
+unsigned xcd_grid(WindowParams& p, int total) {
+    p.total = total;
+    p.run = (total + 7) / 8;
+    if (p.lengths || (p.causal && p.w < 0)) p.run = total / 32 < 1 ? 1 : (total / 32 > 16 ? 16 : total / 32);
+    return (unsigned)((total + 8 * p.run - 1) / (8 * p.run) * 8 * p.run);
+}
 
 template <typename T, int DP, int NW> int run_fwd(WindowParams p, hipStream_t st) {
     constexpr int BK = sizeof(T) == 2 ? 64 : 32;
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
-    p.total = p.B * p.Hq * p.tiles;
+    const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK>), lds);
-    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK>), dim3(grid), dim3(64 * NW), lds, st, p);
     return VITK_OK;
 }
 template <typename T, int DP, int NW> void run_dq(WindowParams p, hipStream_t st) {
     constexpr int BK = sizeof(T) == 2 ? 64 : 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;   // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
-    p.total = p.B * p.Hq * p.tiles;
+    const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK, WPE>), lds);
-    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK, WPE>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK, WPE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
 template <typename T, int DP, int NW, int BQ, bool SINK> void run_dkv(WindowParams p, int tiles, hipStream_t st) {
     // V rows in LDS where they, K's and both accumulators do not fit the registers of two waves a SIMD
     constexpr bool VLDS = sizeof(T) == 2 && DP >= 96 && !SINK;
     constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK ? 1 : 2;
     p.tiles = tiles;
-    p.total = p.B * p.Hk * tiles * (SINK ? p.chunks : 1);
+    const unsigned grid = xcd_grid(p, p.B * p.Hk * tiles * (SINK ? p.chunks : 1));
     const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * NW * DP * sizeof(T) : 0), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tl > rows ? tl : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), lds);
-    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), dim3(xcd_grid(p.total)), dim3(64 * NW), lds, st, p);
+    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
 template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
     constexpr int BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
