@@ -10,6 +10,7 @@
 // a few hundred bytes a token, is shared by the token's heads.  Layout of the work: a "unit" is V pairs, i.e. two
 // chunks of V elements of one row, so both members of each pair sit in one lane whatever the layout of the pairs.  V is
 // 16 bytes' worth where the row's shape and alignment allow it, else 8 bytes' worth, else one element.
+#include <type_traits>
 #include "common.h"
 
 namespace vitk {
@@ -181,7 +182,7 @@ struct Side {                              // queries or keys
     const float* gamma;                    // [dh] or NULL
     void* y;                               // forward: [B][N][H][dh]; backward: dx, the same
     float* part;                           // backward: gamma's partial sums [blocks][dh], or NULL
-    int H, hgroups;
+    int H, hgroups;                        // hgroups = ceil(H / HPT)
     unsigned blocks;                       // workgroups of this side
     unsigned groups;                       // B * N * hgroups
 };
@@ -193,15 +194,24 @@ struct QkNormParams {
     float eps;
 };
 
-template <int V>
+// sum over the row's lanes, in every one of them: lane exchanges on the vector unit (a shuffle would go through LDS)
 __device__ __forceinline__ float row_sum(float v, int lpr_log2) {
-    for (int o = 1; o < (1 << lpr_log2); o <<= 1) v += __shfl_xor(v, o, 64);
+    auto dpp = [](float x, auto ctrl) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    if (lpr_log2 > 0) v += dpp(v, std::integral_constant<int, 0xB1>{});      // quad_perm [1,0,3,2]
+    if (lpr_log2 > 1) v += dpp(v, std::integral_constant<int, 0x4E>{});      // quad_perm [2,3,0,1]
+    if (lpr_log2 > 2) v += dpp(v, std::integral_constant<int, 0x141>{});     // row_half_mirror: the other four of eight
+    if (lpr_log2 > 3) v += dpp(v, std::integral_constant<int, 0x140>{});     // row_mirror: the other eight of sixteen
+    if (lpr_log2 > 4) v += __shfl_xor(v, 16, 64);
+    if (lpr_log2 > 5) v += __shfl_xor(v, 32, 64);
     return v;
 }
 
-// One row (token, head) on 2^lpr_log2 lanes, 256 >> lpr_log2 rows at a time in a workgroup; a group of lanes takes HPT
-// heads of one token in a step.  BWD walks many steps per workgroup so that gamma's sum stays in registers and ends in
-// one partial row per workgroup (a second kernel adds those in a fixed order: no atomics).
+// One row (token, head) on 2^lpr_log2 lanes, 256 >> lpr_log2 of them side by side in a workgroup; a lane group takes HPT
+// heads of one token in a step, so that the token's turn, 8 bytes a pair against 4 or 8 of x, is read once for HPT rows.
+// BWD walks several steps per workgroup so that gamma's sum stays in registers and ends in one partial row per workgroup (a
+// second kernel adds those in a fixed order: no atomics).
 template <typename T, int V, bool INTER, int HPT, bool BWD>
 __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
     const bool isq = blockIdx.x < p.q.blocks;
@@ -256,9 +266,9 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
             chunk_unpack<T, V>(c2[k], f + V);
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) ss += f[i] * f[i];
-            ss = row_sum<V>(ss, p.lpr_log2);
+            ss = row_sum(ss, p.lpr_log2);
             const float r = 1.f / sqrtf(ss * inv + p.eps);
-            T* o = on ? static_cast<T*>(S.y) + ((long)bn * S.H + h0 + k) * p.dh : nullptr;
+            T* o = static_cast<T*>(S.y) + ((long)bn * S.H + h0 + k) * p.dh;
             const bool st = on && h0 + k < S.H;
             if (!BWD) {
 #pragma unroll
@@ -279,7 +289,7 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
                     w[i] *= g[i];
                     tx += w[i] * f[i];
                 }
-                tx = row_sum<V>(tx, p.lpr_log2);
+                tx = row_sum(tx, p.lpr_log2);
                 const float cf = tx * inv * r * r;
 #pragma unroll
                 for (int i = 0; i < 2 * V; ++i) w[i] = r * (w[i] - f[i] * cf);
@@ -291,19 +301,21 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
         }
     }
     if (BWD && S.part) {
-        __shared__ float red[256 * 2 * V];
+        // gamma's sums of the workgroup's lanes: over the slots of one unit, in order, by the threads (part, unit, element)
+        __shared__ float red[2 * V][256];
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) red[i * 256 + threadIdx.x] = acc[i];
+        for (int i = 0; i < 2 * V; ++i) red[i][threadIdx.x] = acc[i];
         __syncthreads();
-        // thread (slot 0, u) adds its unit's sums over the slots, in order
-        if (slot == 0 && live) {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) {
-                if (i >= V && !n2) continue;
-                float t = 0.f;
-                for (int w = 0; w < rows; ++w) t += red[i * 256 + (w << p.lpr_log2) + u];
-                S.part[(long)blk * p.dh + (i < V ? d0 : d1 - V) + i] = t;
-            }
+        for (int e = threadIdx.x; e < 2 * V << p.lpr_log2; e += 256) {
+            const int i = e >> p.lpr_log2, uu = e & ((1 << p.lpr_log2) - 1);
+            if (uu >= p.units) continue;
+            int a0, a1;
+            bool two;
+            unit_at<V, INTER>(uu, p.urot, p.rot, p.dh, a0, a1, two);
+            if (i >= V && !two) continue;
+            float t = 0.f;
+            for (int w = 0; w < rows; ++w) t += red[i][(w << p.lpr_log2) + uu];
+            S.part[(long)blk * p.dh + (i < V ? a0 : a1 - V) + i] = t;
         }
     }
 }
@@ -317,13 +329,18 @@ __global__ __launch_bounds__(256) void qk_norm_dgamma_kernel(const float* pq, co
     if (!out) return;
     const int col = blockIdx.x * 16 + (threadIdx.x & 15), row = threadIdx.x >> 4;
     __shared__ float red[16][17];
-    float t = 0.f;
-    if (col < dh)
-        for (unsigned r = row; r < nb; r += 16) t += part[(long)r * dh + col];
-    red[row][threadIdx.x & 15] = t;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (col < dh) {
+        unsigned r = row;
+        for (; r + 48 < nb; r += 64)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += part[(long)(r + 16 * e) * dh + col];
+        for (; r < nb; r += 16) s[0] += part[(long)r * dh + col];
+    }
+    red[row][threadIdx.x & 15] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
     if (row == 0 && col < dh) {
-        t = 0.f;
+        float t = 0.f;
         for (int r = 0; r < 16; ++r) t += red[r][threadIdx.x & 15];
         out[col] = t;
     }
@@ -363,21 +380,26 @@ void launch_rotary(const RotaryParams& p, bool inter, bool wide, hipStream_t st)
     else { if (wide) GO(false, 4); else GO(false, 1); }
 #undef GO
 }
+// heads a lane takes in a step: as below where the call is large, one where it is small and a step's latency counts
+constexpr int HEADS_FWD = 4, HEADS_BWD = 2;
 template <typename T, int V, bool BWD>
-void launch_qk_norm(const QkNormParams& p, bool inter, bool wide, hipStream_t st) {
+void launch_qk_norm(const QkNormParams& p, bool inter, int hpt, hipStream_t st) {
     const unsigned blocks = p.q.blocks + p.k.blocks;
+    constexpr int W = BWD ? HEADS_BWD : HEADS_FWD;
 #define GO(I, H) hipLaunchKernelGGL((qk_norm_kernel<T, V, I, H, BWD>), dim3(blocks), dim3(256), 0, st, p)
-    if (inter) { if (wide) GO(true, 2); else GO(true, 1); }
-    else { if (wide) GO(false, 2); else GO(false, 1); }
+    if (inter) { if (hpt > 1) GO(true, W); else GO(true, 1); }
+    else { if (hpt > 1) GO(false, W); else GO(false, 1); }
 #undef GO
 }
 
-constexpr unsigned NORM_BLOCKS = 1024;     // backward: workgroups of each side at most (4 a CU), one partial row each
+constexpr unsigned NORM_BLOCKS = 1024;     // backward: workgroups of each side at most, one partial row each
+
+bool large_norm(long B, long N, long H, long dh) { return B * N * H * dh >= 256L * 256 * 64; }     // 64 elements for each of 256 lanes a CU
 
 // the parts of QkNormParams that forward and backward share; returns V, or 0 on an error
 int plan_qk_norm(const char* what, int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
                  const void* k, long kb, long kn, long kh, const float* table, long rows, int rot, const void* ids, int ids64,
-                 long offset, float eps, bool al16, bool al8, bool wide, QkNormParams& p) {
+                 long offset, float eps, bool al16, bool al8, int hpt, QkNormParams& p) {
     const int es = dtype == VITK_F32 ? 4 : 2;
     const int V = chunk_elems(es, dh, rot, al16 && aligned(q, qb, qn, qh, es, 16) && aligned(k, kb, kn, kh, es, 16),
                               al8 && aligned(q, qb, qn, qh, es, 8) && aligned(k, kb, kn, kh, es, 8));
@@ -388,7 +410,6 @@ int plan_qk_norm(const char* what, int dtype, int B, int N, int Hq, int Hk, int 
     p.units = p.urot + (dh - rot + 2 * V - 1) / (2 * V);
     p.lpr_log2 = 0;
     while ((1 << p.lpr_log2) < p.units) ++p.lpr_log2;
-    const int hpt = wide ? 2 : 1;
     Side* s[2] = {&p.q, &p.k};
     const void* x[2] = {q, k};
     const long st[2][3] = {{qb, qn, qh}, {kb, kn, kh}};
@@ -414,7 +435,9 @@ int check_qk_norm(const char* what, int dtype, int B, int N, int Hq, int Hk, int
 unsigned side_blocks(long groups, int lpr_log2, unsigned most) {
     const long per = 256 >> lpr_log2;
     const long b = (groups + per - 1) / per;
-    return (unsigned)(most && b > (long)most ? most : b);
+    if (!most || b <= (long)most) return (unsigned)b;
+    const long steps = (b + most - 1) / most;            // every workgroup takes as many steps as the others, or one less
+    return (unsigned)((b + steps - 1) / steps);
 }
 
 }  // namespace
@@ -464,8 +487,9 @@ extern "C" int vitk_rotary(int dtype, int inverse, int interleaved, int B, int N
     p.urot = rot / 2 / V;
     p.units = p.urot + (dh - rot + 2 * V - 1) / (2 * V);
     p.sgn = inverse ? -1.f : 1.f;
-    // four heads a lane where that still leaves every CU several workgroups; one where the call is small
-    const bool wide = H >= 4 && (long)B * N * H * p.units >= 256L * 256 * 16;
+    // four heads a lane, with one read of the turn for them, where that leaves every CU a workgroup or more (32 x 577 tokens x
+    // 12 heads of 64: 11.8 us, with one head a lane 14.7); one where the call is small
+    const bool wide = H >= 4 && (long)B * N * ((H + 3) / 4) * p.units >= 256L * 256;
     p.hgroups = wide ? (H + 3) / 4 : H;
     const long total = (long)B * N * p.hgroups * p.units;
     VITK_CHECK_ARG(total < (1L << 31) && (long)B * N < (1L << 31), "vitk_rotary: %ld work items are too many for one call", total);
@@ -494,21 +518,21 @@ extern "C" int vitk_qk_norm_rotary_fwd(int dtype, int interleaved, int B, int N,
     VITK_CHECK_ARG(q && k && yq && yk, "%s: null pointer", what);
     const uintptr_t ya = reinterpret_cast<uintptr_t>(yq) | reinterpret_cast<uintptr_t>(yk);
     QkNormParams p = {};
-    const bool wide = (long)B * N * (Hq + Hk) * dh >= 256L * 256 * 64;
+    const int hpt = large_norm(B, N, Hq + Hk, dh) ? HEADS_FWD : 1;
     const int V = plan_qk_norm(what, dtype, B, N, Hq, Hk, dh, q, qb, qn, qh, k, kb, kn, kh, table, table_rows, rot, pos, pos64, offset, eps,
-                               ya % 16 == 0, ya % 8 == 0, wide, p);
+                               ya % 16 == 0, ya % 8 == 0, hpt, p);
     p.q.gamma = gamma_q; p.k.gamma = gamma_k;
     p.q.y = yq; p.k.y = yk;
     p.q.blocks = side_blocks(p.q.groups, p.lpr_log2, 0);
     p.k.blocks = side_blocks(p.k.groups, p.lpr_log2, 0);
     if (dtype == VITK_BF16) {
-        if (V == 8) launch_qk_norm<__bf16, 8, false>(p, interleaved, wide, stream);
-        else if (V == 4) launch_qk_norm<__bf16, 4, false>(p, interleaved, wide, stream);
-        else launch_qk_norm<__bf16, 1, false>(p, interleaved, wide, stream);
+        if (V == 8) launch_qk_norm<__bf16, 8, false>(p, interleaved, hpt, stream);
+        else if (V == 4) launch_qk_norm<__bf16, 4, false>(p, interleaved, hpt, stream);
+        else launch_qk_norm<__bf16, 1, false>(p, interleaved, hpt, stream);
     } else {
-        if (V == 4) launch_qk_norm<float, 4, false>(p, interleaved, wide, stream);
-        else if (V == 2) launch_qk_norm<float, 2, false>(p, interleaved, wide, stream);
-        else launch_qk_norm<float, 1, false>(p, interleaved, wide, stream);
+        if (V == 4) launch_qk_norm<float, 4, false>(p, interleaved, hpt, stream);
+        else if (V == 2) launch_qk_norm<float, 2, false>(p, interleaved, hpt, stream);
+        else launch_qk_norm<float, 1, false>(p, interleaved, hpt, stream);
     }
     VITK_CHECK_LAUNCH(what);
     return VITK_OK;
@@ -535,9 +559,9 @@ extern "C" int vitk_qk_norm_rotary_bwd(int dtype, int interleaved, int B, int N,
         const uintptr_t ya = reinterpret_cast<uintptr_t>(dxq) | reinterpret_cast<uintptr_t>(dxk);
         const bool al16 = ya % 16 == 0 && aligned(dyq, gqb, gqn, gqh, es, 16) && aligned(dyk, gkb, gkn, gkh, es, 16);
         const bool al8 = ya % 8 == 0 && aligned(dyq, gqb, gqn, gqh, es, 8) && aligned(dyk, gkb, gkn, gkh, es, 8);
-        const bool wide = (long)B * N * (Hq + Hk) * dh >= 256L * 256 * 64;
+        const int hpt = large_norm(B, N, Hq + Hk, dh) ? HEADS_BWD : 1;
         const int V = plan_qk_norm(what, dtype, B, N, Hq, Hk, dh, q, qb, qn, qh, k, kb, kn, kh, table, table_rows, rot, pos, pos64,
-                                   offset, eps, al16, al8, wide, p);
+                                   offset, eps, al16, al8, hpt, p);
         p.q.gamma = gamma_q; p.k.gamma = gamma_k;
         p.q.dy = dyq; p.q.gb = gqb; p.q.gn = gqn; p.q.gh = gqh;
         p.k.dy = dyk; p.k.gb = gkb; p.k.gn = gkn; p.k.gh = gkh;
@@ -548,13 +572,13 @@ extern "C" int vitk_qk_norm_rotary_bwd(int dtype, int interleaved, int B, int N,
         p.q.part = dgamma_q ? ws : nullptr;
         p.k.part = dgamma_k ? ws + (long)NORM_BLOCKS * dh : nullptr;
         if (dtype == VITK_BF16) {
-            if (V == 8) launch_qk_norm<__bf16, 8, true>(p, interleaved, wide, stream);
-            else if (V == 4) launch_qk_norm<__bf16, 4, true>(p, interleaved, wide, stream);
-            else launch_qk_norm<__bf16, 1, true>(p, interleaved, wide, stream);
+            if (V == 8) launch_qk_norm<__bf16, 8, true>(p, interleaved, hpt, stream);
+            else if (V == 4) launch_qk_norm<__bf16, 4, true>(p, interleaved, hpt, stream);
+            else launch_qk_norm<__bf16, 1, true>(p, interleaved, hpt, stream);
         } else {
-            if (V == 4) launch_qk_norm<float, 4, true>(p, interleaved, wide, stream);
-            else if (V == 2) launch_qk_norm<float, 2, true>(p, interleaved, wide, stream);
-            else launch_qk_norm<float, 1, true>(p, interleaved, wide, stream);
+            if (V == 4) launch_qk_norm<float, 4, true>(p, interleaved, hpt, stream);
+            else if (V == 2) launch_qk_norm<float, 2, true>(p, interleaved, hpt, stream);
+            else launch_qk_norm<float, 1, true>(p, interleaved, hpt, stream);
         }
     }
     if (any_dg)      // with no rows the sums are zero, and the kernel below writes that

@@ -1105,19 +1105,29 @@ def _unit_heads(t):
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _once(backward):
+    """``backward`` as it is where no graph of it is asked for, else under once_differentiable (which refuses the second
+    derivative, and costs a few microseconds that the ordinary step need not pay)."""
+    refusing = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, table, pos, offset, interleaved):
+        x = _unit_heads(x)
+        ctx.plan = ops.rotary_plan(x, table, pos, offset, interleaved)
         ctx.save_for_backward(table, pos)
-        ctx.cfg = (offset, interleaved)
-        return ops.rotary(_unit_heads(x), table, pos, offset, interleaved)
+        return ops.rotary_run(ctx.plan, x, 0)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        table, pos = ctx.saved_tensors
-        offset, interleaved = ctx.cfg
-        return ops.rotary(_unit_heads(dy), table, pos, offset, interleaved, inverse=True), None, None, None, None
+        ctx.saved_tensors                # alive, and unchanged since
+        return ops.rotary_run(ctx.plan, _unit_heads(dy), 1), None, None, None, None
 
 
 def rotary(x, table, pos=None, offset=0, interleaved=False):
@@ -1131,19 +1141,17 @@ class QkNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
         q, k = _unit_heads(q), _unit_heads(k)
+        ctx.plan = ops.qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
         ctx.save_for_backward(q, k, gamma_q, gamma_k, table, pos)
-        ctx.cfg = (offset, eps, interleaved)
-        return ops.qk_norm_rotary_fwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
+        return ops.qk_norm_rotary_fwd(ctx.plan, q, k)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dq, dk):
-        q, k, gamma_q, gamma_k, table, pos = ctx.saved_tensors
-        offset, eps, interleaved = ctx.cfg
+        ctx.saved_tensors                # alive, and unchanged since
         want = ctx.needs_input_grad
-        dq, dk, dgq, dgk = ops.qk_norm_rotary_bwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved, _unit_heads(dq),
-                                                  _unit_heads(dk), want[2], want[3])
-        return dq, dk, dgq, dgk, None, None, None, None, None
+        grads = ops.qk_norm_rotary_bwd(ctx.plan, _unit_heads(dq), _unit_heads(dk), want[2], want[3])
+        return (*grads, None, None, None, None, None)
 
 
 def qk_norm_rotary(q, k, gamma_q, gamma_k, table=None, pos=None, offset=0, eps=1e-6, interleaved=False):
@@ -1157,20 +1165,19 @@ class WindowAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, causal, scale, lengths):
         q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
+        plan = ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths)
         train = any(ctx.needs_input_grad[:3])
-        out, lse = ops.window_attn_fwd(q, k, v, window, sinks, causal, scale, lengths, want_lse=train)
+        out, lse = ops.window_attn_fwd(plan, q, want_lse=train)
         if train:
+            ctx.plan, ctx.ws_bytes = plan, ops.window_attn_bwd_workspace(plan)
             ctx.save_for_backward(q, k, v, out, lse, lengths)
-            ctx.cfg = (window, sinks, causal, scale)
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
-        window, sinks, causal, scale = ctx.cfg
-        dq, dk, dv = ops.window_attn_bwd(q, k, v, window, sinks, causal, scale, lengths, out, lse, ops._aligned_heads(dout))
-        return dq, dk, dv, None, None, None, None, None
+        _, _, _, out, lse, _ = ctx.saved_tensors
+        return (*ops.window_attn_bwd(ctx.plan, ctx.ws_bytes, out, lse, ops._aligned_heads(dout)), None, None, None, None, None)
 
 
 def window_attention(q, k, v, window, sinks=0, causal=False, scale=None, lengths=None):

@@ -509,12 +509,25 @@ def ce_smooth_bwd(logits, target, smoothing, lse, gout):
 
 
 # ------------------------------------------------------------------ long sequences: rotary positions, window attention
+_get_device = getattr(torch._C, '_cuda_getDevice', None)       # torch.cuda.current_device() without its wrapper
+
+
 def _req_here(*ts):
-    """Every tensor on the current device, where the launch goes."""
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    """Every tensor on the current device, where the launch goes; its index."""
+    dev = None
     for t in ts:
-        if t is not None and not (t.is_cuda and t.get_device() == dev):
-            raise _lib.VitkError('vit_amd ops need tensors on the current GPU (there is no CPU path)')
+        if t is not None:
+            if not t.is_cuda:
+                raise _lib.VitkError('vit_amd ops need tensors on the GPU (there is no CPU path)')
+            if dev is None:
+                dev = _get_device()
+            if t.get_device() != dev:
+                raise _lib.VitkError(f'vit_amd ops need their tensors on the current device, cuda:{dev}')
+    return dev
+
+
+def _stream_on(dev):
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 def _heads(t, what):
@@ -576,18 +589,29 @@ def _turn_args(what, B, N, dh, table, pos, offset):
     return table.data_ptr(), table.shape[0], 2 * table.shape[1], pos.data_ptr(), int(pos.dtype == torch.int64), 0
 
 
+# The autograd Functions check a call once, in the forward (*_plan: sizes, types, pointers of what is kept for the backward),
+# and run it twice: the backward's Python runs in autograd's own thread, where every line of it costs several times more.
+def rotary_plan(x, table, pos, offset, interleaved):
+    dev = _req_here(x, table, pos)
+    (B, N, H, dh), _ = _heads(x, 'rotary x')
+    if table is None:
+        raise ValueError('rotary: no table')
+    return _dt(x), int(interleaved), B, N, H, dh, _turn_args('rotary', B, N, dh, table, pos, offset), dev
+
+
+def rotary_run(plan, x, inverse):
+    dt, inter, B, N, H, dh, turn, dev = plan
+    sb, sn, sh, _ = x.stride()
+    y = x.new_empty((B, N, H, dh))
+    check(lib().vitk_rotary(dt, inverse, inter, B, N, H, dh, x.data_ptr(), sb, sn, sh, *turn, y.data_ptr(), _stream_on(dev)),
+          'vitk_rotary')
+    return y
+
+
 def rotary(x, table, pos=None, offset=0, interleaved=False, inverse=False):
     """Rotary positions on x [B, N, H, dh] (any strides, contiguous heads): a new contiguous tensor.  Token (b, n) takes table row
     pos[b, n], or offset + n; ids outside the table give NaN.  ``inverse``: the adjoint."""
-    _req_here(x, table, pos)
-    (B, N, H, dh), st = _heads(x, 'rotary x')
-    tp, rows, rot, ids, ids64, offset = _turn_args('rotary', B, N, dh, table, pos, offset)
-    if table is None:
-        raise ValueError('rotary: no table')
-    y = torch.empty(B, N, H, dh, device=x.device, dtype=x.dtype)
-    check(lib().vitk_rotary(_dt(x), int(inverse), int(interleaved), B, N, H, dh, x.data_ptr(), st[0], st[1], st[2], tp, rows, rot,
-                            ids, ids64, offset, y.data_ptr(), _stream()), 'vitk_rotary')
-    return y
+    return rotary_run(rotary_plan(x, table, pos, offset, interleaved), x, int(inverse))
 
 
 def _check_qk(q, k, gamma_q, gamma_k):
@@ -601,38 +625,34 @@ def _check_qk(q, k, gamma_q, gamma_k):
     return B, N, Hq, shape[2], dh, sq, sk
 
 
-def qk_norm_rotary_fwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
-    _req_here(q, k, gamma_q, gamma_k, table, pos)
+def qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
+    dev = _req_here(q, k, gamma_q, gamma_k, table, pos)
     B, N, Hq, Hk, dh, sq, sk = _check_qk(q, k, gamma_q, gamma_k)
     turn = _turn_args('qk_norm_rotary', B, N, dh, table, pos, offset)
-    yq = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
-    yk = torch.empty(B, N, Hk, dh, device=q.device, dtype=q.dtype)
-    check(lib().vitk_qk_norm_rotary_fwd(_dt(q), int(interleaved), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2],
-                                        k.data_ptr(), sk[0], sk[1], sk[2], _ptr(gamma_q), _ptr(gamma_k), float(eps), *turn,
-                                        yq.data_ptr(), yk.data_ptr(), _stream()), 'vitk_qk_norm_rotary_fwd')
+    return ((_dt(q), int(interleaved), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
+             _ptr(gamma_q), _ptr(gamma_k), float(eps), *turn), dev)
+
+
+def qk_norm_rotary_fwd(plan, q, k):
+    args, dev = plan
+    yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
+    check(lib().vitk_qk_norm_rotary_fwd(*args, yq.data_ptr(), yk.data_ptr(), _stream_on(dev)), 'vitk_qk_norm_rotary_fwd')
     return yq, yk
 
 
-def qk_norm_rotary_bwd(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved, dyq, dyk, want_dgq, want_dgk):
+def qk_norm_rotary_bwd(plan, dyq, dyk, want_dgq, want_dgk):
     """(dq, dk, dgamma_q, dgamma_k); a gamma gradient that is not wanted is None."""
-    _req_here(q, k, gamma_q, gamma_k, table, pos, dyq, dyk)
-    B, N, Hq, Hk, dh, sq, sk = _check_qk(q, k, gamma_q, gamma_k)
-    turn = _turn_args('qk_norm_rotary', B, N, dh, table, pos, offset)
-    (s1, gq), (s2, gk) = _heads(dyq, 'qk_norm_rotary dq'), _heads(dyk, 'qk_norm_rotary dk')
-    if s1 != q.shape or s2 != k.shape or dyq.dtype != q.dtype or dyk.dtype != q.dtype:
-        raise ValueError('qk_norm_rotary: the gradients must match the outputs')
-    dq = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
-    dk = torch.empty(B, N, Hk, dh, device=q.device, dtype=q.dtype)
-    dgq = torch.empty(dh, device=q.device, dtype=torch.float32) if want_dgq else None
-    dgk = torch.empty(dh, device=q.device, dtype=torch.float32) if want_dgk else None
-    ws = None
+    args, dev = plan
+    dh = args[6]
+    dq, dk = dyq.new_empty(dyq.shape), dyk.new_empty(dyk.shape)
+    dgq = dgk = ws = None
     if want_dgq or want_dgk:
-        ws = torch.empty(lib().vitk_qk_norm_rotary_bwd_workspace_bytes(dh), device=q.device, dtype=torch.uint8)
-    check(lib().vitk_qk_norm_rotary_bwd(_dt(q), int(interleaved), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2],
-                                        k.data_ptr(), sk[0], sk[1], sk[2], _ptr(gamma_q), _ptr(gamma_k), float(eps), *turn,
-                                        dyq.data_ptr(), gq[0], gq[1], gq[2], dyk.data_ptr(), gk[0], gk[1], gk[2],
-                                        dq.data_ptr(), dk.data_ptr(), _ptr(dgq), _ptr(dgk), _ptr(ws), _stream()),
-          'vitk_qk_norm_rotary_bwd')
+        dg = dyq.new_empty((2, dh), dtype=torch.float32)
+        dgq, dgk = dg[0] if want_dgq else None, dg[1] if want_dgk else None
+        ws = dyq.new_empty(lib().vitk_qk_norm_rotary_bwd_workspace_bytes(dh), dtype=torch.uint8)
+    s, r = dyq.stride(), dyk.stride()
+    check(lib().vitk_qk_norm_rotary_bwd(*args, dyq.data_ptr(), s[0], s[1], s[2], dyk.data_ptr(), r[0], r[1], r[2], dq.data_ptr(),
+                                        dk.data_ptr(), _ptr(dgq), _ptr(dgk), _ptr(ws), _stream_on(dev)), 'vitk_qk_norm_rotary_bwd')
     return dq, dk, dgq, dgk
 
 
@@ -659,36 +679,40 @@ def _i32(n):
     return max(-1, min(int(n), 2 ** 31 - 1))
 
 
-def window_attn_fwd(q, k, v, window, sinks, causal, scale, lengths, want_lse=True):
-    """(out [B, N, Hq, dh], lse [B, Hq, N] in log2 or None)."""
-    _req_here(q, k, v, lengths)
+def window_attn_plan(q, k, v, window, sinks, causal, scale, lengths):
+    """q, k, v with 16-byte aligned rows (_aligned_heads)."""
+    dev = _req_here(q, k, v, lengths)
     B, N, Hq, Hk, dh, sq, sk, sv = _check_window(q, k, v, window, sinks, lengths)
-    out = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
-    lse = torch.empty(B, Hq, N, device=q.device, dtype=torch.float32) if want_lse else None
-    check(lib().vitk_window_attn_fwd(_dt(q), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
-                                     v.data_ptr(), sv[0], sv[1], sv[2], float(scale), _i32(window), _i32(sinks), int(causal),
-                                     _ptr(lengths), out.data_ptr(), _ptr(lse), _stream()), 'vitk_window_attn_fwd')
+    return ((_dt(q), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0],
+             sv[1], sv[2], float(scale), _i32(window), _i32(sinks), int(causal), _ptr(lengths)), dev)
+
+
+def window_attn_fwd(plan, q, want_lse=True):
+    """(out [B, N, Hq, dh], lse [B, Hq, N] in log2 or None)."""
+    args, dev = plan
+    B, N, Hq = args[1:4]
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((B, Hq, N), dtype=torch.float32) if want_lse else None
+    check(lib().vitk_window_attn_fwd(*args, out.data_ptr(), lse.data_ptr() if want_lse else 0, _stream_on(dev)),
+          'vitk_window_attn_fwd')
     return out, lse
 
 
-def window_attn_bwd(q, k, v, window, sinks, causal, scale, lengths, out, lse, dout):
+def window_attn_bwd_workspace(plan):
+    """Bytes that window_attn_bwd needs beside its results."""
+    a = plan[0]
+    return lib().vitk_window_attn_bwd_workspace_bytes(*a[:6], a[19], a[20])
+
+
+def window_attn_bwd(plan, ws_bytes, out, lse, dout):
     """(dq, dk, dv), contiguous."""
-    _req_here(q, k, v, lengths, out, lse, dout)
-    B, N, Hq, Hk, dh, sq, sk, sv = _check_window(q, k, v, window, sinks, lengths)
-    shape, so = _heads(dout, 'window_attention dout')
-    if shape != q.shape or dout.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
-        raise ValueError('window_attention: out / dout must match q')
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hq, N) or not lse.is_contiguous():
-        raise ValueError('window_attention: lse must be contiguous fp32 [B, Hq, N]')
-    window, sinks = _i32(window), _i32(sinks)
-    dq = torch.empty(B, N, Hq, dh, device=q.device, dtype=q.dtype)
-    dk, dv = (torch.empty(B, N, Hk, dh, device=q.device, dtype=q.dtype) for _ in range(2))
-    ws = torch.empty(lib().vitk_window_attn_bwd_workspace_bytes(_dt(q), B, N, Hq, Hk, dh, window, sinks), device=q.device,
-                     dtype=torch.uint8)
-    check(lib().vitk_window_attn_bwd(_dt(q), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
-                                     v.data_ptr(), sv[0], sv[1], sv[2], float(scale), window, sinks, int(causal), _ptr(lengths),
-                                     out.data_ptr(), lse.data_ptr(), dout.data_ptr(), so[0], so[1], so[2], dq.data_ptr(),
-                                     dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), _stream()), 'vitk_window_attn_bwd')
+    args, dev = plan
+    B, N, Hq, Hk, dh = args[1:6]
+    dq, dk, dv = dout.new_empty((B, N, Hq, dh)), dout.new_empty((B, N, Hk, dh)), dout.new_empty((B, N, Hk, dh))
+    ws = dout.new_empty(ws_bytes, dtype=torch.uint8)
+    s = dout.stride()
+    check(lib().vitk_window_attn_bwd(*args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), s[0], s[1], s[2], dq.data_ptr(),
+                                     dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), _stream_on(dev)), 'vitk_window_attn_bwd')
     return dq, dk, dv
 
 
@@ -704,7 +728,7 @@ def _check_cache(what, k_cache, v_cache, B, Hk, dh, dtype, lengths):
 def window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks, scale):
     """One new token a sequence: its k / v [B, Hk, dh] into the ring caches (in place), its q [B, Hq, dh] over what is visible:
     out [B, Hq, dh]."""
-    _req_here(q, k, v, k_cache, v_cache, lengths)
+    dev = _req_here(q, k, v, k_cache, v_cache, lengths)
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] \
             or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError('window_decode: q [B, Hq, dh], k and v [B, Hk, dh] of one type expected')
@@ -716,12 +740,12 @@ def window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks, scale):
     q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
     window, sinks = _i32(window), int(sinks)
     L, dt = lib(), _dt(q)
-    out = torch.empty(B, Hq, dh, device=q.device, dtype=q.dtype)
+    out = q.new_empty((B, Hq, dh))
     need = L.vitk_window_decode_workspace_bytes(dt, B, Hq, Hk, dh, C, window, sinks)
-    ws = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     check(L.vitk_window_decode(dt, B, Hq, Hk, dh, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
                                v.data_ptr(), v.stride(0), v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), C,
-                               lengths.data_ptr(), float(scale), window, sinks, out.data_ptr(), _ptr(ws), _stream()),
+                               lengths.data_ptr(), float(scale), window, sinks, out.data_ptr(), _ptr(ws), _stream_on(dev)),
           'vitk_window_decode')
     return out
 
