@@ -29,8 +29,22 @@ struct DecodeParams {
     float sc2;
 };
 
-// the value lane ^ (1 << step) holds, for steps inside a group of lanes
 __device__ __forceinline__ float lane_xor(float v, int m) { return __shfl_xor(v, m, 64); }
+template <int CTRL> __device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+// sum over LPK neighbouring lanes, in every one of them (vector unit up to 16; a shuffle would go through LDS)
+template <int LPK> __device__ __forceinline__ float group_sum(float v) {
+    if (LPK > 1) v += dpp<0xB1>(v);      // quad_perm [1,0,3,2]
+    if (LPK > 2) v += dpp<0x4E>(v);      // quad_perm [2,3,0,1]
+    if (LPK > 4) v += dpp<0x141>(v);     // row_half_mirror
+    if (LPK > 8) v += dpp<0x140>(v);     // row_mirror
+    if (LPK > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    return v;
+}
 
 template <typename T> struct Row16;                       // 16 bytes of a row as floats
 template <> struct Row16<__bf16> { static constexpr int N = 8; };
@@ -42,9 +56,78 @@ template <typename T> __device__ __forceinline__ void unpack16(const u32x4& r, f
     for (int i = 0; i < Row16<T>::N; ++i) f[i] = (float)a.e[i];
 }
 
-template <typename T, int LPK, int GB, int NW>
+// lane g of the row of 16 lanes, to all of them; g: a constant after unrolling
+__device__ __forceinline__ float bcast16(float x, int g) {
+    switch (g) {
+        case 0: return dpp<0x150>(x);    // row_newbcast:0
+        case 1: return dpp<0x151>(x);
+        case 2: return dpp<0x152>(x);
+        case 3: return dpp<0x153>(x);
+        case 4: return dpp<0x154>(x);
+        case 5: return dpp<0x155>(x);
+        case 6: return dpp<0x156>(x);
+        default: return dpp<0x157>(x);
+    }
+}
+
+// the waves' (maximum, sum, vector) of nh query heads, in order, to out or to the split's place
+template <typename T, int GB, int NW, int W>
+__device__ __forceinline__ void join_waves(const DecodeParams& p, const float (&sm)[NW][GB][2], const float (&sv)[NW][GB][W], long row0, int nh,
+                                           int split, bool lost) {
+    for (int x = threadIdx.x; x < nh * p.dh; x += 64 * NW) {
+        const int g = x / p.dh, dd = x - g * p.dh;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][g][0]);
+        float L = 0.f, a = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float mw = sm[w][g][0], lw = sm[w][g][1];
+            const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mw - M);
+            L += lw * f;
+            a += sv[w][g][dd] * f;
+        }
+        const long row = row0 + g;
+        if (p.splits == 1) {
+            const float o = lost ? __builtin_nanf("") : (L == 0.f ? 0.f : a / L);
+            static_cast<T*>(p.out)[row * p.dh + dd] = (T)o;
+        } else {
+            float* w = p.part + (row * p.splits + split) * (2 + p.dh);
+            if (dd == 0) {
+                w[0] = M;
+                w[1] = L;
+            }
+            w[2 + dd] = a;
+        }
+    }
+}
+
+// What sequence b sees, as a list of n tokens: n1 sinks, then lo .. pos.  Slot of entry t: t for the sinks, then a run of the ring
+// that starts at `base` and wraps once at most.
+struct Seen {
+    int n, n1, base, S, R;
+    bool lost;                           // a cache without window is full: NaN out, nothing written
+};
+__device__ __forceinline__ Seen seen_by(const DecodeParams& p, int pos) {
+    Seen s;
+    s.lost = p.w < 0 && pos >= p.C;
+    s.n1 = pos < 0 || s.lost || p.w < 0 ? 0 : min(p.S, pos + 1);
+    const int lo = p.w < 0 ? 0 : max(p.S, pos - p.w);
+    s.n = pos < 0 || s.lost ? 0 : s.n1 + max(0, pos - lo + 1);
+    s.R = p.w < 0 ? p.C : p.C - p.S;
+    s.S = p.w < 0 ? 0 : p.S;
+    s.base = s.n > s.n1 ? (lo - s.S) % s.R : 0;
+    return s;
+}
+__device__ __forceinline__ int seen_slot(const Seen& s, int t) {
+    if (t < s.n1) return t;
+    const int x = s.base + t - s.n1;
+    return s.S + (x >= s.R ? x - s.R : x);
+}
+
+template <typename T, int LPK, int GB, int NW, int U>
 __global__ __launch_bounds__(64 * NW) void window_decode_kernel(const DecodeParams p) {
-    constexpr int E = Row16<T>::N, U = 4;                 // keys in flight a lane group
+    constexpr int E = Row16<T>::N;                        // U: keys in flight a lane group
     constexpr int SLOTS = 64 / LPK, STEP = NW * SLOTS * U;
     __shared__ float sm[NW][GB][2];
     __shared__ float sv[NW][GB][LPK * E];
@@ -60,14 +143,9 @@ __global__ __launch_bounds__(64 * NW) void window_decode_kernel(const DecodePara
     const bool act = c * E < p.dh;
     const int d = act ? c * E : 0;
 
-    const int pos = p.lengths[b];
-    const bool lost = p.w < 0 && pos >= p.C;              // a cache without window is full: NaN out, nothing written
-    // visible tokens: n1 sinks, then lo .. pos
-    const int n1 = pos < 0 || lost || p.w < 0 ? 0 : min(p.S, pos + 1);
-    const int lo = p.w < 0 ? 0 : max(p.S, pos - p.w);
-    const int n = pos < 0 || lost ? 0 : n1 + max(0, pos - lo + 1);
-    const int R = p.w < 0 ? p.C : p.C - p.S, S = p.w < 0 ? 0 : p.S;
-    const int base = n > n1 ? (lo - S) % R : 0;           // ring place of token lo
+    const Seen sn = seen_by(p, p.lengths[b]);
+    const bool lost = sn.lost;
+    const int n = sn.n;
     const T* K = static_cast<const T*>(p.kc) + bh * p.C * p.dh;
     const T* V = static_cast<const T*>(p.vc) + bh * p.C * p.dh;
     const T* kn = static_cast<const T*>(p.k) + b * p.kb + (long)hk * p.kh;
@@ -97,11 +175,7 @@ __global__ __launch_bounds__(64 * NW) void window_decode_kernel(const DecodePara
             ok[u] = t < t1;
             kr[u] = vr[u] = u32x4{0, 0, 0, 0};
             if (ok[u] && act) {
-                int x = (int)t;
-                if (t >= n1) {
-                    x = base + (int)(t - n1);
-                    x = S + (x >= R ? x - R : x);
-                }
+                const int x = seen_slot(sn, (int)t);
                 const bool own = t == n - 1;              // the new token: from the inputs, and into the cache
                 kr[u] = *reinterpret_cast<const u32x4*>(own ? kn + d : K + (long)x * p.dh + d);
                 vr[u] = *reinterpret_cast<const u32x4*>(own ? vn + d : V + (long)x * p.dh + d);
@@ -121,8 +195,7 @@ __global__ __launch_bounds__(64 * NW) void window_decode_kernel(const DecodePara
                 float a = 0.f;
 #pragma unroll
                 for (int e = 0; e < E; ++e) a += q[g][e] * f[e];
-#pragma unroll
-                for (int o = 1; o < LPK; o <<= 1) a += lane_xor(a, o);
+                a = group_sum<LPK>(a);
                 s[u][g] = ok[u] ? a : -INFINITY;
             }
         }
@@ -179,32 +252,166 @@ __global__ __launch_bounds__(64 * NW) void window_decode_kernel(const DecodePara
         }
     }
     __syncthreads();
-    for (int x = threadIdx.x; x < nh * p.dh; x += 64 * NW) {
-        const int g = x / p.dh, dd = x - g * p.dh;
-        float M = -INFINITY;
+    join_waves<T, GB, NW, LPK * E>(p, sm, sv, b * p.Hq + h0, nh, split, lost);
+}
+
+// bf16 and two query heads or more to a key head: the scores of 16 keys and (up to 16) heads are one chain of 16 x 16 x 32
+// MFMA, straight from the cache's rows (a lane holds 16 bytes of key l & 15).  They come out with head l & 15 on the lane and
+// keys 4 (l >> 4) .. + 3 in its registers; V is read so that the same 16 lanes hold those 4 keys' rows, and a probability
+// reaches the row's lanes by a broadcast within 16 lanes.  On the vector unit the scores took 8 products, 8 conversions and
+// 4 exchanges a head and 16 bytes of K: 64 sequences x 4 key heads x 4 x 4100 keys of 128 took 222 us in place of 88 (5.1
+// TB/s, a large copy's rate).
+typedef __attribute__((ext_vector_type(4))) float f32v4;
+template <int LPK, int GB, int NW>
+__global__ __launch_bounds__(64 * NW) void window_decode_group_kernel(const DecodeParams p) {
+    typedef __bf16 T;
+    constexpr int KB = (LPK * 8 + 31) / 32;               // 32-deep K blocks of a row
+    constexpr int KPR = 16 / LPK;                         // keys that 16 lanes read at a time
+    constexpr int U = 2;                                  // tiles of 16 keys in flight a wave
+    constexpr int STEP = NW * 16 * U;
+    __shared__ float sm[NW][GB][2];
+    __shared__ float sv[NW][GB][LPK * 8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = lane >> 4, i = lane & 15;             // 16 lanes: their 4 keys; key (K) / head (scores) / chunk (V)
+    const int c = i % LPK, sub = i / LPK;
+    const int split = blockIdx.x % p.splits;
+    const long r1 = blockIdx.x / p.splits;
+    const int gb = (int)(r1 % p.gblocks);
+    const long bh = r1 / p.gblocks;
+    const int hk = (int)(bh % p.Hk);
+    const long b = bh / p.Hk;
+    const int h0 = hk * p.G + gb * GB, nh = min(GB, p.G - gb * GB);
+    const bool act = c * 8 < p.dh;
+
+    const Seen sn = seen_by(p, p.lengths[b]);
+    const T* K = static_cast<const T*>(p.kc) + bh * p.C * p.dh;
+    const T* V = static_cast<const T*>(p.vc) + bh * p.C * p.dh;
+    const T* kn = static_cast<const T*>(p.k) + b * p.kb + (long)hk * p.kh;
+    const T* vn = static_cast<const T*>(p.v) + b * p.vb + (long)hk * p.vh;
+    bf16x8 qf[KB];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w][g][0]);
-        float L = 0.f, a = 0.f;
+    for (int kb = 0; kb < KB; ++kb) {
+        const int d = 32 * kb + 8 * row;
+        u32x4 r = {0, 0, 0, 0};
+        if (i < nh && d < p.dh) r = *reinterpret_cast<const u32x4*>(static_cast<const T*>(p.q) + b * p.qb + (long)(h0 + i) * p.qh + d);
+        qf[kb] = __builtin_bit_cast(bf16x8, r);
+    }
+    float acc[GB][8], m = -INFINITY, l = 0.f;             // m, l: head i's, over this row of lanes' keys
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float mw = sm[w][g][0], lw = sm[w][g][1];
-            const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mw - M);
-            L += lw * f;
-            a += sv[w][g][dd] * f;
-        }
-        const long row = b * p.Hq + h0 + g;
-        if (p.splits == 1) {
-            const float o = lost ? __builtin_nanf("") : (L == 0.f ? 0.f : a / L);
-            static_cast<T*>(p.out)[row * p.dh + dd] = (T)o;
-        } else {
-            float* w = p.part + (row * p.splits + split) * (2 + p.dh);
-            if (dd == 0) {
-                w[0] = M;
-                w[1] = L;
+    for (int g = 0; g < GB; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[g][e] = 0.f;
+
+    const long t0 = split * p.keys_per_split, t1 = min((long)sn.n, t0 + p.keys_per_split);
+    for (long tt = t0 + 16 * U * wave; tt < t1; tt += STEP) {     // the same for the whole wave
+        u32x4 kr[U][KB], vr[U][4 / KPR];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long t = tt + 16 * u + i;
+            const bool own = t == sn.n - 1;               // the new token: from the inputs, and into the cache
+            const long x = t < t1 ? seen_slot(sn, (int)t) : 0;
+            const T* from = own ? kn : K + x * p.dh;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const int d = 32 * kb + 8 * row;
+                kr[u][kb] = u32x4{0, 0, 0, 0};
+                if (t < t1 && d < p.dh) {
+                    kr[u][kb] = *reinterpret_cast<const u32x4*>(from + d);
+                    if (own && gb == 0) *reinterpret_cast<u32x4*>(static_cast<T*>(p.kc) + (bh * p.C + x) * p.dh + d) = kr[u][kb];
+                }
             }
-            w[2 + dd] = a;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4 / KPR; ++j) {
+                const long t = tt + 16 * u + 4 * row + KPR * j + sub;
+                vr[u][j] = u32x4{0, 0, 0, 0};
+                if (t < t1 && act) {
+                    const bool own = t == sn.n - 1;
+                    const long x = seen_slot(sn, (int)t);
+                    vr[u][j] = *reinterpret_cast<const u32x4*>((own ? vn : V + x * p.dh) + 8 * c);
+                    if (own && gb == 0) *reinterpret_cast<u32x4*>(static_cast<T*>(p.vc) + (bh * p.C + x) * p.dh + 8 * c) = vr[u][j];
+                }
+            }
+        f32v4 s[U];
+        float mt = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = f32v4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[u][kb]), qf[kb], s[u], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[u][r] = tt + 16 * u + 4 * row + r < t1 ? s[u][r] * p.sc2 : -INFINITY;
+                mt = fmaxf(mt, s[u][r]);
+            }
+        }
+        if (__any(mt > m + 8.f)) {                        // the reference point moves with 2^8, as in the prefill
+            const float mn = fmaxf(m, mt);
+            const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int g = 0; g < GB; ++g) {
+                const float ag = bcast16(al, g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[g][e] *= ag;
+            }
+        }
+        const float mr = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - mr);
+                l += s[u][r];
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4 / KPR; ++j) {
+                float f[8];
+                unpack16<T>(vr[u][j], f);
+#pragma unroll
+                for (int g = 0; g < GB; ++g) {
+                    float pk[KPR], pg;                    // the broadcasts need all 16 lanes: no choice around them
+#pragma unroll
+                    for (int k = 0; k < KPR; ++k) pk[k] = bcast16(s[u][KPR * j + k], g);
+                    pg = pk[0];
+#pragma unroll
+                    for (int k = 1; k < KPR; ++k) pg = sub == k ? pk[k] : pg;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[g][e] += pg * f[e];
+                }
+            }
+    }
+    // join the wave's 4 rows of lanes (and the keys that shared one), then the waves
+    float M = m;
+    M = fmaxf(M, lane_xor(M, 16));
+    M = fmaxf(M, lane_xor(M, 32));
+    const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M);
+    l *= f;
+    l += lane_xor(l, 16);
+    l += lane_xor(l, 32);
+    if (lane < nh) {
+        sm[wave][lane][0] = M;
+        sm[wave][lane][1] = l;
+    }
+#pragma unroll
+    for (int g = 0; g < GB; ++g) {
+        const float fg = bcast16(f, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            acc[g][e] *= fg;
+#pragma unroll
+            for (int o = LPK; o < 64; o <<= 1) acc[g][e] += lane_xor(acc[g][e], o);
+            if (lane < LPK) sv[wave][g][lane * 8 + e] = acc[g][e];
         }
     }
+    __syncthreads();
+    join_waves<T, GB, NW, LPK * 8>(p, sm, sv, b * p.Hq + h0, nh, split, sn.lost);
 }
 
 // joins the splits of one (sequence, query head), in order
@@ -277,22 +484,27 @@ bool al16(const void* p, int es, long a, long b = 0, long c = 0) {
 }
 
 struct DecodePlan { int splits, gb, gblocks, nw; long per; };
+// Waves a workgroup and workgroups a row (sequence, key head, up to 4 query heads).  Up to 256 KiB of keys and values a row is
+// one workgroup's work, of 16 waves where there are few rows: a second kernel costs more than it saves.  Beyond, keys are
+// dealt to so many workgroups that every CU has 8 waves or more (256 rows of 4100 keys of 128, bf16, groups of 4: 88 us with
+// one workgroup of 8 waves a row, 96 with two and the join, 129 with 16 waves, whose registers spill).
 DecodePlan decode_plan(int B, int Hq, int Hk, int dh, int C, int w, int S, int es) {
     DecodePlan d;
     const int G = Hq / Hk;
+    const bool group = es == 2 && G > 1;
     d.gb = G == 1 ? 1 : (G == 2 ? 2 : 4);
     d.gblocks = (G + d.gb - 1) / d.gb;
     const long most = w < 0 ? C : (long)S + w + 1;
     const long rows = (long)B * Hk * d.gblocks, bytes = most * dh * es * 2;
-    d.nw = 4;
+    const int few = group ? 8 : 16;
     long splits = 1;
-    if (rows * 4 < 1024 && bytes > 256 * 1024) {
-        splits = (1024 + rows - 1) / rows;
+    d.nw = rows < 512 ? few : 4;
+    if (rows < 192 && bytes > 256 * 1024) {
+        d.nw = group ? 8 : 4;
+        splits = (2048 / d.nw + rows - 1) / rows;
         const long cap = (bytes + 64 * 1024 - 1) / (64 * 1024);
         if (splits > cap) splits = cap;
         if (splits > 64) splits = 64;
-    } else if (rows < 512) {
-        d.nw = 16;
     }
     d.splits = (int)splits;
     d.per = (most + splits - 1) / splits;
@@ -300,13 +512,23 @@ DecodePlan decode_plan(int B, int Hq, int Hk, int dh, int C, int w, int S, int e
 }
 
 template <typename T, int LPK, int GB> void launch_decode(const DecodeParams& p, int nw, long blocks, hipStream_t st) {
-    if (nw == 4) hipLaunchKernelGGL((window_decode_kernel<T, LPK, GB, 4>), dim3((unsigned)blocks), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((window_decode_kernel<T, LPK, GB, 16>), dim3((unsigned)blocks), dim3(1024), 0, st, p);
+    if (nw == 4) hipLaunchKernelGGL((window_decode_kernel<T, LPK, GB, 4, 4>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((window_decode_kernel<T, LPK, GB, 16, 4>), dim3((unsigned)blocks), dim3(1024), 0, st, p);
+}
+template <int LPK, int GB> void launch_group(const DecodeParams& p, int nw, long blocks, hipStream_t st) {
+    if (nw == 4) hipLaunchKernelGGL((window_decode_group_kernel<LPK, GB, 4>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((window_decode_group_kernel<LPK, GB, 8>), dim3((unsigned)blocks), dim3(512), 0, st, p);
 }
 template <typename T, int LPK> void decode_heads(const DecodeParams& p, const DecodePlan& d, long blocks, hipStream_t st) {
-    if (d.gb == 1) launch_decode<T, LPK, 1>(p, d.nw, blocks, st);
-    else if (d.gb == 2) launch_decode<T, LPK, 2>(p, d.nw, blocks, st);
-    else launch_decode<T, LPK, 4>(p, d.nw, blocks, st);
+    if constexpr (sizeof(T) == 2) {
+        if (d.gb == 1) launch_decode<T, LPK, 1>(p, d.nw, blocks, st);
+        else if (d.gb == 2) launch_group<LPK, 2>(p, d.nw, blocks, st);
+        else launch_group<LPK, 4>(p, d.nw, blocks, st);
+    } else {
+        if (d.gb == 1) launch_decode<T, LPK, 1>(p, d.nw, blocks, st);
+        else if (d.gb == 2) launch_decode<T, LPK, 2>(p, d.nw, blocks, st);
+        else launch_decode<T, LPK, 4>(p, d.nw, blocks, st);
+    }
 }
 
 }  // namespace
