@@ -257,15 +257,38 @@ __device__ __forceinline__ RowRange row_range(const WindowParams& p, int i, int 
     r.s = min(p.S, e + 1);
     return r;
 }
-// for a wave's queries [i, i + BQ) and keys [j0, j0 + BK): 0 nothing visible, 1 some, 2 all
+// What a wave's queries [i, i + BQ) see of keys [j0, j0 + BK): NOTHING, ALL, or which of its edges the test has to look at
+enum { NOTHING = 0, ALL = 1, EDGE_HI = 2, EDGE_LO = 4, EDGE_ANY = 8 };
 __device__ __forceinline__ int tile_kind(const WindowParams& p, int i, int BQ, int j0, int BK, int len) {
-    if (i >= len) return 0;
+    if (i >= len) return NOTHING;
     const int j1 = j0 + BK - 1, i1 = i + BQ - 1;
-    if (p.causal && j0 > i1) return 0;
+    if (p.causal && j0 > i1) return NOTHING;
     const bool in = p.w < 0 || (j1 >= i - p.w && j0 <= i1 + p.w);
-    if (!in && j0 >= p.S) return 0;
-    const bool all = (p.w < 0 || (j0 >= i1 - p.w && j1 <= i + p.w) || j1 < p.S) && (!p.causal || j1 <= i) && j1 < len;
-    return all ? 2 : 1;
+    if (!in && j0 >= p.S) return NOTHING;
+    const bool hi = j1 >= len || (p.causal && j1 > i) || (p.w >= 0 && j1 > i + p.w), lo = p.w >= 0 && j0 < i1 - p.w;
+    if (j1 < p.S && j1 < len && (!p.causal || j1 <= i)) return ALL;
+    if (j0 < p.S && (hi || lo)) return EDGE_ANY;
+    return hi ? (lo ? EDGE_ANY : EDGE_HI) : (lo ? EDGE_LO : ALL);
+}
+// scores of keys j0 .. that query (rr) does not see become -inf (S^T: register e of sub-tile u is key 32 u + 8 (e >> 2) + 4
+// (lane >> 5) + (e & 3))
+template <int NS>
+__device__ __forceinline__ void hide(f32x16 (&s)[NS], int kind, const RowRange& rr, int j0, int lane) {
+    const int lo = rr.lo - j0 - 4 * (lane >> 5), hi = lo + (int)rr.span, sk = rr.s - j0 - 4 * (lane >> 5);
+#define VITK_HIDE(COND)                                                      \
+    _Pragma("unroll") for (int u = 0; u < NS; ++u)                           \
+    _Pragma("unroll") for (int e = 0; e < 16; ++e) {                         \
+        const int c = 32 * u + 8 * (e >> 2) + (e & 3);                       \
+        s[u][e] = (COND) ? s[u][e] : -INFINITY;                              \
+    }
+    if (kind == EDGE_HI) {
+        VITK_HIDE(c <= hi)
+    } else if (kind == EDGE_LO) {
+        VITK_HIDE(c >= lo)
+    } else {
+        VITK_HIDE((unsigned)(c - lo) <= rr.span || c < sk)
+    }
+#undef VITK_HIDE
 }
 
 // ---------------------------------------------------------------------------------------------------------- forward
@@ -329,23 +352,14 @@ __global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowPara
             for (int u = 0; u < NS; ++u) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
+                Frag<T> ka[KD];                           // all on their way before the first product (4 % at 128 wide heads)
 #pragma unroll
-                for (int kk = 0; kk < KD; ++kk) {
-                    Frag<T> a;
-                    row_frag32<DP>(a, Ks, 32 * u, kk, lane);
-                    s[u] = mma32(a, qf[kk], s[u]);
-                }
+                for (int kk = 0; kk < KD; ++kk) row_frag32<DP>(ka[kk], Ks, 32 * u, kk, lane);
+                if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int kk = 0; kk < KD; ++kk) s[u] = mma32(ka[kk], qf[kk], s[u]);
             }
-            if (kind == 1) {
-#pragma unroll
-                for (int u = 0; u < NS; ++u)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int j = j0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                        const bool ok = (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
-                        s[u][e] = ok ? s[u][e] : -INFINITY;
-                    }
-            }
+            if (kind != ALL) hide(s, kind, rr, j0, lane);
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
@@ -493,7 +507,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.sc2, -lse)) * (dp[e] - delta);
-                if (kind == 1) {
+                if (kind != ALL) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const int j = j0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
@@ -563,7 +577,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
     int ta = 0, nt = 0;
     if (j0 < len) {
         int a = p.causal ? j0 : 0, e = len;
-        if (!SINK && p.w >= 0) {
+        if (p.w >= 0 && j0 >= p.S) {                     // (the sinks' tiles are seen from everywhere)
             a = max(a, j0 - p.w);
             e = (int)min((long)e, (long)j0 + 32 * NW + p.w);
         }
@@ -629,7 +643,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
                 s[4 * q + e] = pe;
             }
         }
-        if (kind == 1) {                                 // (no second copy of the products: it costs moves of all accumulators)
+        if (kind != ALL) {                               // (no second copy of the products: it costs moves of all accumulators)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const bool ok = (unsigned)(i0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) - ilo) <= span;
@@ -685,29 +699,32 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
     put_rows<T, DP>(dv, 1.f, j >= len, mine, static_cast<T*>(p.dv) + at, ldg, jw, p.N, p.dh, lane);
 }
 
-// rows of the sinks' tiles: the shares' sum in order, rounded once.  A workgroup takes 8 head elements of one (sequence, key
-// head, tile), dk or dv: 32 keys x 8 elements, one a thread, so its reads are whole rows of the partial sums.
+// rows of the sinks' tiles: the shares' sum in a fixed order, rounded once.  A workgroup takes 2 head elements of one (sequence,
+// key head, tile), dk or dv, times 32 keys; each of its waves a quarter of the shares.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void window_sink_sum_kernel(const WindowParams p) {
-    __shared__ float t[32][9];
-    const int d0 = 8 * (blockIdx.x % (DP / 8)), which = blockIdx.x / (DP / 8) % 2;
-    const long set = blockIdx.x / (DP / 8) / 2;
-    const int tk = (int)(set % p.tiles), bh = (int)(set / p.tiles);
-    const int b = bh / p.Hk, hk = bh % p.Hk;
+    __shared__ float t[4][64];
+    const int d0 = 2 * (blockIdx.x % (DP / 2)), which = blockIdx.x / (DP / 2) % 2;
+    const int set = blockIdx.x / (DP / 2) / 2;
+    const int bh = set / p.tiles, tk = set - bh * p.tiles;
+    const int b = bh / p.Hk, hk = bh - b * p.Hk;
     if (d0 >= p.dh) return;
-    const float* part = p.part + (set * p.chunks * 2 + which) * DP * 32 + d0 * 32 + threadIdx.x;
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, per = (p.chunks + 3) / 4;
+    const float* from = p.part + ((long)set * p.chunks * 2 + which) * DP * 32 + d0 * 32 + lane;
+    const int c1 = min(p.chunks, (part + 1) * per);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    int c = 0;
-    for (; c + 8 <= p.chunks; c += 8)
+    int c = part * per;
+    for (; c + 8 <= c1; c += 8)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += part[(long)(c + e) * 2 * DP * 32];
-    for (; c < p.chunks; ++c) s[0] += part[(long)c * 2 * DP * 32];
-    const float sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
-    t[threadIdx.x & 31][threadIdx.x >> 5] = which ? sum : sum * p.scale;
+        for (int e = 0; e < 8; ++e) s[e] += from[(long)(c + e) * 2 * DP * 32];
+    for (; c < c1; ++c) s[0] += from[(long)c * 2 * DP * 32];
+    t[part][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
-    const int r = threadIdx.x >> 3, d = d0 + (threadIdx.x & 7), j = 32 * tk + r;
-    T* out = static_cast<T*>(which ? p.dv : p.dk);
-    if (j < p.N) out[(((long)b * p.N + j) * p.Hk + hk) * p.dh + d] = (T)t[r][threadIdx.x & 7];
+    const int j = 32 * tk + (lane >> 1), at = 32 * (lane & 1) + (lane >> 1);     // two neighbours hold one key's two elements
+    if (part == 0 && j < p.N) {
+        const float sum = (t[0][at] + t[1][at]) + (t[2][at] + t[3][at]);
+        static_cast<T*>(which ? p.dv : p.dk)[(((long)b * p.N + j) * p.Hk + hk) * p.dh + d0 + (lane & 1)] = (T)(which ? sum : sum * p.scale);
+    }
 }
 
 }  // namespace vitk
@@ -723,16 +740,20 @@ struct Plan {                  // tiles of one call
     int chunks, per_chunk;
 };
 constexpr int SINK_BQ = 32;
+constexpr int NARROW = 128;
 
 // Fewer, larger workgroups read K and V fewer times; they are halved where the large ones would leave CUs without work.
 int waves_for(long rows_tiles_of_128) { return rows_tiles_of_128 >= 512 ? 4 : 2; }
 
-Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S) {
+Plan make_plan(int B, int N, int Hq, int Hk, int dh, int w, int S) {
     Plan pl;
     pl.dp = (dh + 31) / 32 * 32;
     pl.nwq = waves_for((long)B * Hq * ((N + 127) / 128));
     pl.nwk = waves_for((long)B * Hk * ((N + 127) / 128));
-    pl.sink_keys = w >= 0 && S > 0 ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
+    // The sinks' keys are seen by all N queries, other keys by 2 w + 1: where that is over four times more, they get a launch of
+    // their own, whose workgroups share the queries; else they stay in the ordinary one (16 x 577 tokens, window 64: 45 us in
+    // all against 33 + 14 + 7).
+    pl.sink_keys = w >= 0 && S > 0 && N > 4L * (128 + 2L * w) ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
     pl.chunks = pl.per_chunk = 0;
     if (pl.sink_keys) {
         // about 1024 one-wave workgroups, at least 4 query tiles each
@@ -783,18 +804,24 @@ unsigned xcd_grid(WindowParams& p, int total) {
     return (unsigned)((total + 8 * p.run - 1) / (8 * p.run) * 8 * p.run);
 }
 
-template <typename T, int DP, int NW> int run_fwd(WindowParams p, hipStream_t st) {
-    constexpr int BK = sizeof(T) == 2 ? 64 : 32;
+template <typename T, int DP, int NW, int BK> void run_fwd(WindowParams p, hipStream_t st) {
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK>), lds);
     hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK>), dim3(grid), dim3(64 * NW), lds, st, p);
-    return VITK_OK;
+}
+// Key tiles of 64 in bf16; of 32 where the window is narrow and a tile of 64 would be mostly edge (16 x 577 tokens x 12 heads
+// of 64: window 64 on both sides 22.6 us against 26.5; causal window of 512 55 against 53, of 1024 222 against 190).
+template <typename T, int DP, int NW> void run_fwd(const WindowParams& p, hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.w < 0 || p.w > NARROW) return run_fwd<T, DP, NW, 64>(p, st);
+    }
+    run_fwd<T, DP, NW, 32>(p, st);
 }
 template <typename T, int DP, int NW> void run_dq(WindowParams p, hipStream_t st) {
-    constexpr int BK = sizeof(T) == 2 ? 64 : 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;   // one wave a SIMD where two would spill
+    constexpr int BK = 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;   // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
@@ -825,7 +852,7 @@ template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void*
         s.per_chunk = pl.per_chunk;
         run_dkv<T, DP, 1, SINK_BQ, true>(s, pl.sink_keys / 32, st);
         s.tiles = pl.sink_keys / 32;
-        hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles * 2 * (DP / 8))), dim3(256),
+        hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles * 2 * (DP / 2))), dim3(256),
                            0, st, s);
     }
     p.key0 = pl.sink_keys;
@@ -855,7 +882,7 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, causal, scale, lengths);
     p.out = out;
     p.lse = lse;
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
     VITK_CHECK_ARG((long)B * Hq * ((N + 63) / 64) < (1L << 30), "%s: too many tiles for one call", what);
 #define GO(T, D) if (pl.nwq == 4) run_fwd<T, D, 4>(p, stream); else run_fwd<T, D, 2>(p, stream)
 #define BY_DP(T) switch (pl.dp) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 96: GO(T, 96); break; default: GO(T, 128); break; }
@@ -870,7 +897,7 @@ extern "C" long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, in
     if (B <= 0 || N <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || dh < 8 || dh > 128 || sinks < 0) return 0;
     WindowParams p = {};
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, 0, 1.f, nullptr);
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
     return ((long)B * Hq * N + 3) / 4 * 16 + part_floats(pl, B, Hk) * 4;
 }
 
@@ -903,7 +930,7 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     p.part = p.delta + ((long)B * Hq * N + 3) / 4 * 4;
     p.dk = dk;
     p.dv = dv;
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
 #define GO(T, D) run_bwd<T, D>(p, pl, dq, stream)
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
     else { BY_DP(float) }
