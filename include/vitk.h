@@ -300,14 +300,18 @@ int vitk_qk_norm_rotary_bwd(int dtype, int interleaved, int B, int N, int Hq, in
  * window < 0: every key.  Query head h reads key head h / (Hq / Hk).  lengths (int32 [B], may be NULL): tokens of each padded
  * sequence; rows past it are not read, their outputs and gradients are 0.  dh: a multiple of 8 up to 128; pointers and strides
  * 16-byte aligned.  lse [B][Hq][N] fp32 (may be NULL in a forward without backward): log2 of the softmax sum, +inf for a row that
- * sees nothing (its output is 0).  The backward sums nothing with atomics. */
+ * sees nothing (its output is 0).  out_lo (bf16, like out, may be NULL): what the rounding took from out, for the backward of
+ * the same call (which then has o . do to 2^-16).  The backward sums nothing with atomics.  Forward: a row depends on nothing
+ * that it does not see, NaN and infinities included; backward: a non-finite value of a token within the lengths can reach the
+ * gradients of the 128 tokens next to those that see it. */
 int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
                          const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
-                         int window, int sinks, int causal, const int* lengths, void* out, float* lse, void* stream);
+                         int window, int sinks, int causal, const int* lengths, void* out, void* out_lo, float* lse,
+                         void* stream);
 long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, int Hq, int Hk, int dh, int window, int sinks);
 int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
                          const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
-                         int window, int sinks, int causal, const int* lengths, const void* out, const float* lse,
+                         int window, int sinks, int causal, const int* lengths, const void* out, const void* out_lo, const float* lse,
                          const void* dout, long ob, long on, long oh, void* dq, void* dk, void* dv, void* workspace, void* stream);
 /* One new token a sequence: its k / v [B][Hk][dh] go into the ring cache [B][Hk][C][dh] (token p in slot p for p < sinks, else
  * sinks + (p - sinks) % (C - sinks)) and its q [B][Hq][dh] attends (causal, as above) to what is visible there.  lengths

@@ -138,6 +138,26 @@ def test_minus_infinity_scores():
     assert torch.allclose(o[0, :, 0].double(), P @ v[0, :, 0].double(), atol=1e-4)
 
 
+@pytest.mark.parametrize('causal', [False, True], ids=['both', 'causal'])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('window', [3, 40, 150])
+def test_a_row_depends_on_nothing_that_it_does_not_see(window, dtype, causal):
+    """NaN and infinities in some tokens' k and v: the rows that do not see them are the same bits or, where a tile was shared,
+    within the bounds; rows that see one are not finite."""
+    from vit_amd import functional as VF
+    g = _gen(20)
+    N, sinks = 400, 2
+    q, k, v = (t.clone() for t in _qkv(g, dtype, 1, N, 2, 1, 64))
+    want = R.window_attention(q, k, v, window, sinks, causal, 0.125, None)['o']
+    for j, t, x in ((100, v, float('nan')), (130, v, float('inf')), (260, k, float('nan')), (261, v, float('-inf'))):
+        t[0, j] = x
+    o = VF.window_attention(q, k, v, window, sinks=sinks, causal=causal)
+    seen = R.visible(N, window, sinks, causal, N, 'cuda')[:, [100, 130, 260, 261]].any(1)
+    assert not torch.isfinite(o[0, seen]).any()
+    assert torch.isfinite(o[0, ~seen]).all()
+    R.within(o[:, ~seen], want[0][:, ~seen], want[1][:, ~seen], 'unseen')
+
+
 def test_same_bits_again_and_two_streams():
     from vit_amd import functional as VF
     g = _gen(17)

@@ -47,7 +47,7 @@ def test_norm_refusals(L, kw, words):
 
 
 def window(L, dtype=BF16, B=1, N=16, Hq=4, Hk=2, dh=64, q=P, st=(8192, 512, 64), scale=0.125, w=4, sinks=1, out=P):
-    return L.vitk_window_attn_fwd(dtype, B, N, Hq, Hk, dh, q, *st, P, 8192, 512, 64, P, 8192, 512, 64, scale, w, sinks, 0, 0, out, 0, 0)
+    return L.vitk_window_attn_fwd(dtype, B, N, Hq, Hk, dh, q, *st, P, 8192, 512, 64, P, 8192, 512, 64, scale, w, sinks, 0, 0, out, 0, 0, 0)
 
 
 @pytest.mark.parametrize('kw,words', [
@@ -63,7 +63,7 @@ def test_window_refusals(L, kw, words):
 def test_window_backward_refusals(L):
     def call(lse=P, ws=P, dq=P, on=512):
         return L.vitk_window_attn_bwd(BF16, 1, 16, 4, 2, 64, P, 8192, 512, 64, P, 8192, 512, 64, P, 8192, 512, 64, 0.125, 4, 1, 0, 0,
-                                      P, lse, P, 8192, on, 64, dq, P, P, ws, 0)
+                                      P, 0, lse, P, 8192, on, 64, dq, P, P, ws, 0)
     _bad(L, call(lse=0), 'null')
     _bad(L, call(ws=0), 'null')
     _bad(L, call(ws=P + 8), 'aligned')

@@ -86,10 +86,10 @@ _SIGNATURES = {
                                 + [c_vp, c_vp, c_float, c_vp, c_long, c_int, c_vp, c_int, c_long]
                                 + [c_vp, c_long, c_long, c_long] * 2 + [c_vp] * 6, c_int),
     'vitk_window_attn_fwd': ([c_int] * 6 + [c_vp, c_long, c_long, c_long] * 3
-                             + [c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp], c_int),
+                             + [c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp], c_int),
     'vitk_window_attn_bwd_workspace_bytes': ([c_int] * 8, c_long),
     'vitk_window_attn_bwd': ([c_int] * 6 + [c_vp, c_long, c_long, c_long] * 3
-                             + [c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_long, c_long, c_long]
+                             + [c_float, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_long, c_long, c_long]
                              + [c_vp] * 5, c_int),
     'vitk_window_decode_workspace_bytes': ([c_int] * 8, c_long),
     'vitk_window_decode': ([c_int] * 5 + [c_vp, c_long, c_long] * 3

@@ -94,6 +94,7 @@ struct View {                     // element (b, n, h, d) at b*sb + n*sn + h*sh 
 struct WindowParams {
     View q, k, v, dout;           // dout: backward
     const void* o;                // backward: the forward's output, [B][N][Hq][dh]
+    void* o_lo;                   // bf16, or NULL: what rounding took from o, rounded itself; the forward writes it, D reads it
     void *out, *dk, *dv;          // out: o in the forward, dq in the queries' backward kernel; all [B][N][H][dh]
     float* lse;                   // [B][Hq][N]: log2 of the softmax sum, maximum included; +inf where a row sees nothing
     float* delta;                 // [B][Hq][N]: D_i, written by the queries' kernel for the keys' kernel
@@ -188,20 +189,24 @@ __device__ __forceinline__ float half_sum(float x) {
     return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
 }
 
-// this wave's 32 rows of a strided matrix as fragments (rows outside [0, hi) are zero)
+// this wave's 32 rows of a strided matrix as fragments (rows outside [0, hi) are zero).  Loads without a branch, so that all are
+// on their way together: a lane with nothing to read reads the first element and drops it.
 template <typename T, int DP>
 __device__ __forceinline__ void own_rows(Frag<T> (&f)[DP / 16], const T* g, long sn, int row, int hi, int dh, int lane) {
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
         const int d = 16 * kk + 8 * (lane >> 5);
-        if (row < hi && d < dh) frag_load(f[kk], g + (long)row * sn + d);
-        else frag_zero(f[kk]);
+        frag_load(f[kk], g + (row < hi && d < dh ? (long)row * sn + d : 0));
     }
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+        if (!(row < hi && 16 * kk + 8 * (lane >> 5) < dh)) frag_zero(f[kk]);
 }
 
 // X^T[d][row] (a lane owns a row) times `mul` -> rows [row0, row0 + 32) of [.][dh] with row stride ldg, turned in LDS so
-// that the stores are whole chunks; rows >= hi are not written.  Only this wave's part of LDS is used.
-template <typename T, int DP>
+// that the stores are whole chunks; rows >= hi are not written.  Only this wave's part of LDS is used.  REST: what the
+// rounding to T leaves over, rounded to T.
+template <typename T, int DP, bool REST = false>
 __device__ __forceinline__ void put_rows(const f32x16 (&x)[DP / 32], float mul, bool zero, T* lds, T* g, long ldg, int row0, int hi, int dh,
                                          int lane) {
     using C = WCfg<T, DP>;
@@ -212,7 +217,11 @@ __device__ __forceinline__ void put_rows(const f32x16 (&x)[DP / 32], float mul, 
         for (int q = 0; q < 4; ++q) {
             T4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(zero ? 0.f : x[t][4 * q + e] * mul);
+            for (int e = 0; e < 4; ++e) {
+                float y = zero ? 0.f : x[t][4 * q + e] * mul;
+                if (REST) y -= (float)(T)y;
+                v[e] = (T)y;
+            }
             *reinterpret_cast<T4*>(lds + (lane & 31) * C::LD + 32 * t + 8 * q + 4 * (lane >> 5)) = v;
         }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -417,10 +426,56 @@ __global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowPara
     }
     const float l = half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
     const bool none = i >= len || (m == -INFINITY && l == 0.f);      // nothing visible (a NaN sum stays a NaN)
+    // A non-finite V of a key that only some queries of a tile see has reached the others as 0 * V.  Where the result is not
+    // finite, it is made again key by key, for the keys that each query sees.
+    float bad = 0.f;
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) bad += o[t][e] * 0.f;
+    if (__any(!none && bad != 0.f)) {                    // (a NaN is unequal)
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+        const int first = p.w < 0 ? 0 : max(0, iw - p.w), last = min(len, p.causal ? iw + 32 : (p.w < 0 ? len : iw + 32 + p.w));
+        const int sinks = min(p.S, len);
+        const float mr = m == -INFINITY ? 0.f : m;
+        for (int x = 0; x < sinks + max(0, last - first); ++x) {
+            const int j = x < sinks ? x : first + x - sinks;
+            if (x >= sinks && j < sinks) continue;       // a sink: had its turn
+            float s = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KD; ++kk) {
+                const int d = 16 * kk + 8 * (lane >> 5);
+                if (d < p.dh) {
+                    Frag<T> a;
+                    frag_load(a, K + (long)j * p.k.sn + d);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s += frag_get_f(a, e) * frag_get_f(qf[kk], e);
+                }
+            }
+            s = half_sum(s) * p.sc2;
+            const bool ok = (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
+            const float pj = __builtin_amdgcn_exp2f(s - mr);
+#pragma unroll
+            for (int t = 0; t < ND; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int d = 32 * t + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                    if (d < p.dh) {
+                        const float y = o[t][e] + pj * to_f32(V[(long)j * p.v.sn + d]);
+                        o[t][e] = ok ? y : o[t][e];
+                    }
+                }
+        }
+    }
     if (p.lse && lane < 32 && i < p.N) p.lse[((long)b * p.Hq + h) * p.N + i] = none ? INFINITY : m + __log2f(l);
     __syncthreads();
-    put_rows<T, DP>(o, 1.f / l, none, lds + wave * 32 * C::LD, static_cast<T*>(p.out) + ((long)b * p.N * p.Hq + h) * p.dh,
-                    (long)p.Hq * p.dh, iw, p.N, p.dh, lane);
+    const long at = ((long)b * p.N * p.Hq + h) * p.dh, ldg = (long)p.Hq * p.dh;
+    T* mine = lds + wave * 32 * C::LD;
+    put_rows<T, DP>(o, 1.f / l, none, mine, static_cast<T*>(p.out) + at, ldg, iw, p.N, p.dh, lane);
+    if (sizeof(T) == 2 && p.o_lo) put_rows<T, DP, true>(o, 1.f / l, none, mine, static_cast<T*>(p.o_lo) + at, ldg, iw, p.N, p.dh, lane);
 }
 
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
@@ -447,16 +502,19 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     own_rows<T, DP>(df, static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i, len, p.dh, lane);
     float delta = 0.f, lse = INFINITY;
     {
-        const T* O = static_cast<const T*>(p.o) + ((long)b * p.N * p.Hq + h) * p.dh;
+        // with o as it was rounded, D's error is the same for all of a row's keys and reaches dq and dk whole: as much again as
+        // the rounding of dS where a row sees few keys
+        const long row = ((long)b * p.N * p.Hq + h) * p.dh;
+        Frag<T> of[KD], lo[KD];
+        own_rows<T, DP>(of, static_cast<const T*>(p.o) + row, (long)p.Hq * p.dh, i, len, p.dh, lane);
+        if (sizeof(T) == 2 && p.o_lo) own_rows<T, DP>(lo, static_cast<const T*>(p.o_lo) + row, (long)p.Hq * p.dh, i, len, p.dh, lane);
 #pragma unroll
-        for (int kk = 0; kk < KD; ++kk) {
-            Frag<T> of[1];
-            const int d = 16 * kk + 8 * (lane >> 5);
-            if (i < len && d < p.dh) frag_load(of[0], O + (long)i * p.Hq * p.dh + d);
-            else frag_zero(of[0]);
+        for (int kk = 0; kk < KD; ++kk)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta += frag_get_f(of[0], e) * frag_get_f(df[kk], e);
-        }
+            for (int e = 0; e < 8; ++e) {
+                const float x = frag_get_f(of[kk], e), d = frag_get_f(df[kk], e);
+                delta += (sizeof(T) == 2 && p.o_lo ? x + frag_get_f(lo[kk], e) : x) * d;
+            }
         delta = half_sum(delta);
         const long at = ((long)b * p.Hq + h) * p.N + i;
         if (i < len) lse = p.lse[at];
@@ -867,7 +925,8 @@ template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void*
 
 extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
                                     const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
-                                    int window, int sinks, int causal, const int* lengths, void* out, float* lse, hipStream_t stream) {
+                                    int window, int sinks, int causal, const int* lengths, void* out, void* out_lo, float* lse,
+                                    hipStream_t stream) {
     const char* what = "vitk_window_attn_fwd";
     if (int e = check_window(what, dtype, B, N, Hq, Hk, dh, scale, sinks)) return e;
     if (B == 0 || N == 0) return VITK_OK;
@@ -878,9 +937,11 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     if (int e = check_view(what, "q", p.q, dtype)) return e;
     if (int e = check_view(what, "k", p.k, dtype)) return e;
     if (int e = check_view(what, "v", p.v, dtype)) return e;
-    VITK_CHECK_ARG(out && (reinterpret_cast<uintptr_t>(out) & 15) == 0, "%s: out must be 16-byte aligned", what);
+    VITK_CHECK_ARG(out && ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo)) & 15) == 0,
+                   "%s: out must be 16-byte aligned", what);
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, causal, scale, lengths);
     p.out = out;
+    p.o_lo = out_lo;
     p.lse = lse;
     const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
     VITK_CHECK_ARG((long)B * Hq * ((N + 63) / 64) < (1L << 30), "%s: too many tiles for one call", what);
@@ -903,7 +964,7 @@ extern "C" long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, in
 
 extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
                                     const void* k, long kb, long kn, long kh, const void* v, long vb, long vn, long vh, float scale,
-                                    int window, int sinks, int causal, const int* lengths, const void* out, const float* lse,
+                                    int window, int sinks, int causal, const int* lengths, const void* out, const void* out_lo, const float* lse,
                                     const void* dout, long ob, long on, long oh, void* dq, void* dk, void* dv, void* workspace,
                                     hipStream_t stream) {
     const char* what = "vitk_window_attn_bwd";
@@ -919,12 +980,13 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     if (int e = check_view(what, "v", p.v, dtype)) return e;
     if (int e = check_view(what, "dout", p.dout, dtype)) return e;
     VITK_CHECK_ARG(out && lse && dq && dk && dv && workspace, "%s: null pointer", what);
-    VITK_CHECK_ARG(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) |
+    VITK_CHECK_ARG(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo) | reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) |
                      reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
                    "%s: out, dq, dk, dv and the workspace must be 16-byte aligned", what);
     VITK_CHECK_ARG((long)B * Hq * ((N + 63) / 64) < (1L << 30), "%s: too many tiles for one call", what);
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, causal, scale, lengths);
     p.o = out;
+    p.o_lo = const_cast<void*>(out_lo);
     p.lse = const_cast<float*>(lse);
     p.delta = static_cast<float*>(workspace);
     p.part = p.delta + ((long)B * Hq * N + 3) / 4 * 4;

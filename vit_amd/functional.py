@@ -1167,17 +1167,17 @@ class WindowAttentionFn(torch.autograd.Function):
         q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
         plan = ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths)
         train = any(ctx.needs_input_grad[:3])
-        out, lse = ops.window_attn_fwd(plan, q, want_lse=train)
+        out, lse, lo = ops.window_attn_fwd(plan, q, train)
         if train:
             ctx.plan, ctx.ws_bytes = plan, ops.window_attn_bwd_workspace(plan)
-            ctx.save_for_backward(q, k, v, out, lse, lengths)
+            ctx.save_for_backward(q, k, v, out, lse, lo, lengths)
         return out
 
     @staticmethod
     @_once
     def backward(ctx, dout):
-        _, _, _, out, lse, _ = ctx.saved_tensors
-        return (*ops.window_attn_bwd(ctx.plan, ctx.ws_bytes, out, lse, ops._aligned_heads(dout)), None, None, None, None, None)
+        _, _, _, out, lse, lo, _ = ctx.saved_tensors
+        return (*ops.window_attn_bwd(ctx.plan, ctx.ws_bytes, out, lse, lo, ops._aligned_heads(dout)), None, None, None, None, None)
 
 
 def window_attention(q, k, v, window, sinks=0, causal=False, scale=None, lengths=None):

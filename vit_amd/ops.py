@@ -687,15 +687,16 @@ def window_attn_plan(q, k, v, window, sinks, causal, scale, lengths):
              sv[1], sv[2], float(scale), _i32(window), _i32(sinks), int(causal), _ptr(lengths)), dev)
 
 
-def window_attn_fwd(plan, q, want_lse=True):
-    """(out [B, N, Hq, dh], lse [B, Hq, N] in log2 or None)."""
+def window_attn_fwd(plan, q, train=True):
+    """(out [B, N, Hq, dh], lse [B, Hq, N] in log2, out_lo): lse and, in bf16, what out's rounding took (out_lo) are for the
+    backward, None without ``train``."""
     args, dev = plan
     B, N, Hq = args[1:4]
     out = q.new_empty(q.shape)
-    lse = q.new_empty((B, Hq, N), dtype=torch.float32) if want_lse else None
-    check(lib().vitk_window_attn_fwd(*args, out.data_ptr(), lse.data_ptr() if want_lse else 0, _stream_on(dev)),
-          'vitk_window_attn_fwd')
-    return out, lse
+    lse = q.new_empty((B, Hq, N), dtype=torch.float32) if train else None
+    lo = q.new_empty(q.shape) if train and args[0] == BF16 else None
+    check(lib().vitk_window_attn_fwd(*args, out.data_ptr(), _ptr(lo), _ptr(lse), _stream_on(dev)), 'vitk_window_attn_fwd')
+    return out, lse, lo
 
 
 def window_attn_bwd_workspace(plan):
@@ -704,14 +705,14 @@ def window_attn_bwd_workspace(plan):
     return lib().vitk_window_attn_bwd_workspace_bytes(*a[:6], a[19], a[20])
 
 
-def window_attn_bwd(plan, ws_bytes, out, lse, dout):
+def window_attn_bwd(plan, ws_bytes, out, lse, lo, dout):
     """(dq, dk, dv), contiguous."""
     args, dev = plan
     B, N, Hq, Hk, dh = args[1:6]
     dq, dk, dv = dout.new_empty((B, N, Hq, dh)), dout.new_empty((B, N, Hk, dh)), dout.new_empty((B, N, Hk, dh))
     ws = dout.new_empty(ws_bytes, dtype=torch.uint8)
     s = dout.stride()
-    check(lib().vitk_window_attn_bwd(*args, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), s[0], s[1], s[2], dq.data_ptr(),
+    check(lib().vitk_window_attn_bwd(*args, out.data_ptr(), _ptr(lo), lse.data_ptr(), dout.data_ptr(), s[0], s[1], s[2], dq.data_ptr(),
                                      dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), _stream_on(dev)), 'vitk_window_attn_bwd')
     return dq, dk, dv
 
