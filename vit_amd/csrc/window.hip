@@ -121,25 +121,16 @@ __device__ __forceinline__ int xcd_order(int total, int run) {
 }
 
 // BYTES a lane from a buffer (voff: the lane's byte offset; past the end reads as 0) to dst + BYTES * lane in LDS, without waiting:
-// tile_ready() does.  In assembly (there is no result register that could be reused too early), because the compiler takes
-// the transpose reads of the present tile for readers of whatever the builtin is writing, and waits for the next tile in
-// front of them.  m0 is the LDS address; it wants one wait state before its use, and nothing else in these kernels uses it.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
+// tile_ready() does.  (The compiler waits for these in front of transpose reads, which it takes for readers of what is being
+// written; written in assembly, which it does not wait for, they were no faster.)
 template <int BYTES> __device__ __forceinline__ void load_to_lds(const void* base, unsigned bytes, unsigned voff, void* dst) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    typedef __attribute__((ext_vector_type(4))) unsigned rsrc_t;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(base);
-    const rsrc_t rs = {(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32) & 0xffffu),
-                       (unsigned)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
-    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>(dst));
-    if constexpr (BYTES == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(voff), "s"(rs) : "memory", "m0");
-    else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(voff), "s"(rs) : "memory", "m0");
+#if defined(__HIP_DEVICE_COMPILE__)       // the host's pass does not know the 16-byte form
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+    if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(uintptr_t)dst, 16, voff, 0, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(uintptr_t)dst, 4, voff, 0, 0, 0);
 #endif
 }
-#pragma clang diagnostic pop
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }     // vmcnt(0), in a form the compiler counts
 
 // Rows [row0, row0 + ROWS) of a strided matrix into an image, asynchronously and without passing through registers; rows outside
@@ -301,8 +292,8 @@ __device__ __forceinline__ void hide(f32x16 (&s)[NS], int kind, const RowRange& 
 }
 
 // ---------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DP, int NW, int BK>
-__global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowParams p) {
+template <typename T, int DP, int NW, int BK, int WPE>
+__global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -361,12 +352,12 @@ __global__ __launch_bounds__(64 * NW, 2) void window_fwd_kernel(const WindowPara
             for (int u = 0; u < NS; ++u) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
-                Frag<T> ka[KD];                           // all on their way before the first product (4 % at 128 wide heads)
 #pragma unroll
-                for (int kk = 0; kk < KD; ++kk) row_frag32<DP>(ka[kk], Ks, 32 * u, kk, lane);
-                if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int kk = 0; kk < KD; ++kk) s[u] = mma32(ka[kk], qf[kk], s[u]);
+                for (int kk = 0; kk < KD; ++kk) {
+                    Frag<T> a;
+                    row_frag32<DP>(a, Ks, 32 * u, kk, lane);
+                    s[u] = mma32(a, qf[kk], s[u]);
+                }
             }
             if (kind != ALL) hide(s, kind, rr, j0, lane);
 #pragma unroll
@@ -863,12 +854,13 @@ unsigned xcd_grid(WindowParams& p, int total) {
 }
 
 template <typename T, int DP, int NW, int BK> void run_fwd(WindowParams p, hipStream_t st) {
+    constexpr int WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;           // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK>), lds);
-    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK>), dim3(grid), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK, WPE>), lds);
+    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK, WPE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
 // Key tiles of 64 in bf16; of 32 where the window is narrow and a tile of 64 would be mostly edge (16 x 577 tokens x 12 heads
 // of 64: window 64 on both sides 22.6 us against 26.5; causal window of 512 55 against 53, of 1024 222 against 190).
@@ -879,7 +871,7 @@ template <typename T, int DP, int NW> void run_fwd(const WindowParams& p, hipStr
     run_fwd<T, DP, NW, 32>(p, st);
 }
 template <typename T, int DP, int NW> void run_dq(WindowParams p, hipStream_t st) {
-    constexpr int BK = 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;   // one wave a SIMD where two would spill
+    constexpr int BK = 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
