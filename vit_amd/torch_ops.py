@@ -12,6 +12,10 @@ without any of that state: tensors in, tensors out, compute dtype = the dtype of
     attention(qkv[B*N,3D], tables[2N-1,2D]?, B, N, H, scale, band) -> (out[B*N,D], lse fp32[B,H,N])
     label_smoothing_ce(logits fp32[B,C], target int64[B], smoothing) -> loss fp32[]
     allreduce_bucket(flat (mutated), scale) -> ()      the gradient exchange of one flat bucket (RCCL sum, then * scale)
+    rotary(x[B,N,H,dh], table, pos[B,N]?, offset, interleaved) -> y
+    qk_norm_rotary(q, k, gamma_q?, gamma_k?, table?, pos?, offset, eps, interleaved) -> (q', k')
+    window_attention(q[B,N,Hq,dh], k, v[B,N,Hk,dh], window, sinks, causal, scale, lengths[B]?) -> (out, lse fp32[B,Hq,N], out_lo)
+    window_decode(q[B,Hq,dh], k, v[B,Hk,dh], k_cache, v_cache (mutated), lengths, window, sinks, scale) -> out
 
 Reference surfaces: nn.Linear / nn.LayerNorm calls of the encoder layers (model.py:183-204), AttentionLAI.forward
 (timm_classes/timm_locality_aware_transformer.py:45-79) and DisentangledSelfAttention.forward
@@ -221,3 +225,145 @@ def allreduce_bucket(flat: Tensor, scale: float) -> None:
 @allreduce_bucket.register_fake
 def _(flat, scale):
     return None
+
+
+# ------------------------------------------------------- long sequences: rotary positions, window attention, its cache
+def _contiguous_like(x):
+    return x.new_empty(x.shape)
+
+
+def _unit(t):
+    """Contiguous heads, as the kernels read them."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+@torch.library.custom_op('vit_amd::rotary', mutates_args=(), device_types='cuda')
+def rotary(x: Tensor, table: Tensor, pos: Optional[Tensor], offset: int, interleaved: bool) -> Tensor:
+    return ops.rotary(_unit(x), table, pos, offset, interleaved)
+
+
+@rotary.register_fake
+def _(x, table, pos, offset, interleaved):
+    return _contiguous_like(x)
+
+
+@torch.library.custom_op('vit_amd::rotary_backward', mutates_args=(), device_types='cuda')
+def rotary_backward(dy: Tensor, table: Tensor, pos: Optional[Tensor], offset: int, interleaved: bool) -> Tensor:
+    return ops.rotary(_unit(dy), table, pos, offset, interleaved, inverse=True)
+
+
+@rotary_backward.register_fake
+def _(dy, table, pos, offset, interleaved):
+    return _contiguous_like(dy)
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, table, pos, offset, interleaved = inputs
+    ctx.save_for_backward(table, pos)
+    ctx.cfg = (offset, interleaved)
+
+
+def _rotary_backward(ctx, dy):
+    table, pos = ctx.saved_tensors
+    return torch.ops.vit_amd.rotary_backward(dy, table, pos, *ctx.cfg), None, None, None, None
+
+
+rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+
+@torch.library.custom_op('vit_amd::qk_norm_rotary', mutates_args=(), device_types='cuda')
+def qk_norm_rotary(q: Tensor, k: Tensor, gamma_q: Optional[Tensor], gamma_k: Optional[Tensor], table: Optional[Tensor],
+                   pos: Optional[Tensor], offset: int, eps: float, interleaved: bool) -> Tuple[Tensor, Tensor]:
+    q, k = _unit(q), _unit(k)
+    return ops.qk_norm_rotary_fwd(ops.qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved), q, k)
+
+
+@qk_norm_rotary.register_fake
+def _(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
+    return _contiguous_like(q), _contiguous_like(k)
+
+
+@torch.library.custom_op('vit_amd::qk_norm_rotary_backward', mutates_args=(), device_types='cuda')
+def qk_norm_rotary_backward(dyq: Tensor, dyk: Tensor, q: Tensor, k: Tensor, gamma_q: Optional[Tensor], gamma_k: Optional[Tensor],
+                            table: Optional[Tensor], pos: Optional[Tensor], offset: int, eps: float,
+                            interleaved: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    q, k = _unit(q), _unit(k)
+    plan = ops.qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
+    dq, dk, dgq, dgk = ops.qk_norm_rotary_bwd(plan, _unit(dyq), _unit(dyk), True, True)
+    return dq, dk, dgq.clone(), dgk.clone()                  # custom-op outputs may not alias each other
+
+
+@qk_norm_rotary_backward.register_fake
+def _(dyq, dyk, q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
+    dh = q.shape[-1]
+    return (_contiguous_like(q), _contiguous_like(k), q.new_empty(dh, dtype=torch.float32), q.new_empty(dh, dtype=torch.float32))
+
+
+def _norm_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:6])
+    ctx.cfg = inputs[6:]
+
+
+def _norm_backward(ctx, dyq, dyk):
+    q, k, gamma_q, gamma_k, table, pos = ctx.saved_tensors
+    dq, dk, dgq, dgk = torch.ops.vit_amd.qk_norm_rotary_backward(dyq, dyk, q, k, gamma_q, gamma_k, table, pos, *ctx.cfg)
+    return (dq, dk, None if gamma_q is None else dgq, None if gamma_k is None else dgk, None, None, None, None, None)
+
+
+qk_norm_rotary.register_autograd(_norm_backward, setup_context=_norm_setup)
+
+
+@torch.library.custom_op('vit_amd::window_attention', mutates_args=(), device_types='cuda')
+def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, causal: bool, scale: float,
+                     lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    """out_lo: what bf16's rounding took from out, for the backward (empty in fp32)."""
+    q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
+    out, lse, lo = ops.window_attn_fwd(ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths), q)
+    return out, lse, q.new_empty(0) if lo is None else lo
+
+
+@window_attention.register_fake
+def _(q, k, v, window, sinks, causal, scale, lengths):
+    lo = _contiguous_like(q) if q.dtype == torch.bfloat16 else q.new_empty(0)
+    return _contiguous_like(q), q.new_empty(q.shape[0], q.shape[2], q.shape[1], dtype=torch.float32), lo
+
+
+@torch.library.custom_op('vit_amd::window_attention_backward', mutates_args=(), device_types='cuda')
+def window_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, out_lo: Tensor, window: int,
+                              sinks: int, causal: bool, scale: float,
+                              lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
+    plan = ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths)
+    return ops.window_attn_bwd(plan, ops.window_attn_bwd_workspace(plan), out, lse, out_lo if out_lo.numel() else None,
+                               ops._aligned_heads(dout))
+
+
+@window_attention_backward.register_fake
+def _(dout, q, k, v, out, lse, out_lo, window, sinks, causal, scale, lengths):
+    return _contiguous_like(q), _contiguous_like(k), _contiguous_like(v)
+
+
+def _window_setup(ctx, inputs, output):
+    q, k, v, window, sinks, causal, scale, lengths = inputs
+    ctx.save_for_backward(q, k, v, *output, lengths)
+    ctx.cfg = (window, sinks, causal, scale)
+
+
+def _window_backward(ctx, dout, dlse, dlo):
+    q, k, v, out, lse, lo, lengths = ctx.saved_tensors
+    dq, dk, dv = torch.ops.vit_amd.window_attention_backward(dout, q, k, v, out, lse, lo, *ctx.cfg, lengths)
+    return dq, dk, dv, None, None, None, None, None
+
+
+window_attention.register_autograd(_window_backward, setup_context=_window_setup)
+
+
+@torch.library.custom_op('vit_amd::window_decode', mutates_args=('k_cache', 'v_cache'), device_types='cuda')
+def window_decode(q: Tensor, k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, window: int, sinks: int,
+                  scale: float) -> Tensor:
+    return ops.window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks, scale)
+
+
+@window_decode.register_fake
+def _(q, k, v, k_cache, v_cache, lengths, window, sinks, scale):
+    return _contiguous_like(q)
