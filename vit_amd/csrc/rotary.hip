@@ -51,27 +51,40 @@ __device__ __forceinline__ long pos_row(const Pos& p, long bn, int n) {
     return p.ids64 ? (long)static_cast<const long long*>(p.ids)[bn] : (long)static_cast<const int*>(p.ids)[bn];
 }
 
-// V (cos, sin) pairs of unit u of table row `row`
-template <int V> __device__ __forceinline__ void load_turn(const float* table, long row, long rows, int pairs, int u, float* c, float* s) {
-    if (row < 0 || row >= rows) {
+// n (cos, sin) pairs from pair `at` of a table row on
+template <int N> __device__ __forceinline__ void load_pairs(const float* row, int at, float* c, float* s) {
+    const float* t = row + 2 * at;
+    if (N % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) c[i] = s[i] = __builtin_nanf("");
-        return;
-    }
-    const float* t = table + 2 * (row * pairs + (long)u * V);
-    if (V % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < V; i += 2) {
+        for (int i = 0; i < N; i += 2) {
             const f32x4 w = *reinterpret_cast<const f32x4*>(t + 2 * i);
             c[i] = w[0]; s[i] = w[1]; c[i + 1] = w[2]; s[i + 1] = w[3];
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) { c[i] = t[2 * i]; s[i] = t[2 * i + 1]; }
+        for (int i = 0; i < N; ++i) { c[i] = t[2 * i]; s[i] = t[2 * i + 1]; }
     }
 }
 
-// f[0..V) and f[V..2V): the unit's two chunks (halves of V pairs, or 2V consecutive elements when interleaved)
+// A unit's two chunks are V elements at u and V elements half the rotated width further on, whichever way the pairs lie: a
+// chunk with its partner (halves), or two chunks of V / 2 pairs each (interleaved), so that neighbouring lanes read
+// neighbouring chunks either way.  (Single elements, interleaved: the pair itself.)
+template <int V, bool INTER> __device__ __forceinline__ void load_turn(const float* table, long row, long rows, int pairs, int u, float* c, float* s) {
+    if (row < 0 || row >= rows) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = s[i] = __builtin_nanf("");
+        return;
+    }
+    const float* t = table + 2 * row * pairs;
+    if (INTER && V > 1) {
+        load_pairs<V / 2>(t, V / 2 * u, c, s);
+        load_pairs<V / 2>(t, pairs / 2 + V / 2 * u, c + V / 2, s + V / 2);
+    } else {
+        load_pairs<V>(t, V * u, c, s);
+    }
+}
+
+// f[0..V) and f[V..2V): the unit's two chunks
 template <int V, bool INTER> __device__ __forceinline__ void turn(float* f, const float* c, const float* s) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -82,16 +95,16 @@ template <int V, bool INTER> __device__ __forceinline__ void turn(float* f, cons
     }
 }
 
-// element offsets of a unit's two chunks within the row; n2: whether the second one exists (the last unit of an
-// unrotated tail may be a single chunk)
-template <int V, bool INTER> __device__ __forceinline__ void unit_at(int u, int urot, int rot, int dh, int& d0, int& d1, bool& n2) {
+// element offsets of a unit's two chunks within the row; n2: whether the second one exists (an unrotated tail may have an odd
+// number of chunks)
+template <int V, bool INTER> __device__ __forceinline__ void unit_at(int u, int urot, int units, int rot, int dh, int& d0, int& d1, bool& n2) {
     n2 = true;
     if (u < urot) {
-        d0 = INTER ? 2 * V * u : V * u;
-        d1 = INTER ? d0 + V : d0 + rot / 2;
+        d0 = INTER && V == 1 ? 2 * u : V * u;
+        d1 = INTER && V == 1 ? d0 + 1 : d0 + rot / 2;
     } else {
-        d0 = rot + 2 * V * (u - urot);
-        d1 = d0 + V;
+        d0 = rot + V * (u - urot);
+        d1 = d0 + V * (units - urot);
         n2 = d1 < dh;
     }
 }
@@ -141,7 +154,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
     T* y = static_cast<T*>(p.y) + ((long)bn * p.H + h0) * p.dh;
     int d0, d1;
     bool n2;
-    unit_at<V, INTER>(u, p.urot, p.rot, p.dh, d0, d1, n2);
+    unit_at<V, INTER>(u, p.urot, p.units, p.rot, p.dh, d0, d1, n2);
     typename Chunk<T, V>::R a[HPT], c2[HPT];
 #pragma unroll
     for (int k = 0; k < HPT; ++k)
@@ -151,7 +164,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
         }
     float c[V], s[V];
     if (u < p.urot) {
-        load_turn<V>(p.table, pos_row(p.pos, bn, n), p.pos.rows, p.rot / 2, u, c, s);
+        load_turn<V, INTER>(p.table, pos_row(p.pos, bn, n), p.pos.rows, p.rot / 2, u, c, s);
 #pragma unroll
         for (int i = 0; i < V; ++i) s[i] *= p.sgn;
     }
@@ -222,7 +235,7 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
     const bool live = u < p.units;
     int d0 = 0, d1 = 0;
     bool n2 = false;
-    if (live) unit_at<V, INTER>(u, p.urot, p.rot, p.dh, d0, d1, n2);
+    if (live) unit_at<V, INTER>(u, p.urot, p.units, p.rot, p.dh, d0, d1, n2);
     float g[2 * V], acc[2 * V];
 #pragma unroll
     for (int i = 0; i < 2 * V; ++i) {
@@ -253,7 +266,7 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
                         if (n2) gc[k] = chunk_load<T, V>(dy + k * S.gh + d1);
                     }
                 }
-            if (u < p.urot) load_turn<V>(p.table, pos_row(p.pos, bn, n), p.pos.rows, p.rot / 2, u, c, s);
+            if (u < p.urot) load_turn<V, INTER>(p.table, pos_row(p.pos, bn, n), p.pos.rows, p.rot / 2, u, c, s);
             if (BWD) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) s[i] = -s[i];
@@ -311,7 +324,7 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
             if (uu >= p.units) continue;
             int a0, a1;
             bool two;
-            unit_at<V, INTER>(uu, p.urot, p.rot, p.dh, a0, a1, two);
+            unit_at<V, INTER>(uu, p.urot, p.units, p.rot, p.dh, a0, a1, two);
             if (i >= V && !two) continue;
             float t = 0.f;
             for (int w = 0; w < rows; ++w) t += red[i][(w << p.lpr_log2) + uu];
