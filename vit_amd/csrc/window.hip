@@ -104,6 +104,7 @@ struct WindowParams {
     int w, S, causal;
     int tiles;                    // query tiles / key tiles of a sequence
     int key0;                     // keys' kernel: first key (the sinks before it have their own launch)
+    int heavy;                    // keys' kernel: how many of a sequence's tiles, the first ones, hold sinks
     int chunks, per_chunk;        // sinks' launch: query tiles are dealt to `chunks` workgroups
     int run;                      // consecutive pieces of work an XCD takes at a time
     int total;                    // workgroups that have work (the grid is rounded up to whole rounds of the 8 XCDs)
@@ -114,9 +115,9 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 
 // Workgroups are dealt to the 8 XCDs in turn.  Neighbours in the work (same keys, other head of the group; next tile) should
 // share an L2, so an XCD takes runs of `run` consecutive pieces of work.
-__device__ __forceinline__ int xcd_order(int total, int run) {
-    const int slot = (int)(blockIdx.x >> 3), r = uniform(slot / run);
-    const int id = (r * 8 + (int)(blockIdx.x & 7)) * run + slot - r * run;
+__device__ __forceinline__ int xcd_order(int block, int total, int run) {
+    const int slot = block >> 3, r = uniform(slot / run);
+    const int id = (r * 8 + (block & 7)) * run + slot - r * run;
     return id < total ? id : -1;
 }
 
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (K tile, V tile)
-    const int id = xcd_order(p.total, p.run);
+    const int id = xcd_order((int)blockIdx.x, p.total, p.run);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // order of the work: the group's heads, then query tiles, then (sequence, key head); causal: long rows first
@@ -476,7 +477,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);
-    const int id = xcd_order(p.total, p.run);
+    const int id = xcd_order((int)blockIdx.x, p.total, p.run);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r1 = uniform(id / p.G), g = id - r1 * p.G;
@@ -594,16 +595,27 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (Q tile, dO tile), then of BQ (lse, D) each
     float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
-    const int id = xcd_order(p.total, p.run);
+    // tiles with sinks in an ordinary launch take longest and go first, one to each XCD in turn
+    const int first = p.heavy * p.B * p.Hk, round = (first + 7) / 8 * 8;
+    int id, chunk = 0, bh, tk;
+    if ((int)blockIdx.x < round) {
+        id = (int)blockIdx.x < first ? (int)blockIdx.x : -1;
+        bh = uniform((int)blockIdx.x / max(p.heavy, 1));
+        tk = (int)blockIdx.x - bh * p.heavy;
+    } else {
+        id = xcd_order((int)blockIdx.x - round, p.total, p.run);
+        int r1 = max(id, 0);
+        if (SINK) {
+            chunk = r1;
+            r1 = uniform(r1 / p.chunks);
+            chunk -= r1 * p.chunks;
+        }
+        const int rest = p.tiles - p.heavy;
+        bh = uniform(r1 / rest);
+        tk = p.heavy + r1 - bh * rest;
+    }
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int chunk = 0;
-    int r1 = id;
-    if (SINK) {
-        r1 = uniform(id / p.chunks);
-        chunk = id - r1 * p.chunks;
-    }
-    const int bh = uniform(r1 / p.tiles), tk = r1 - bh * p.tiles;
     const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk;
     const int j0 = p.key0 + 32 * NW * tk, jw = j0 + 32 * wave, j = jw + (lane & 31);
     const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
@@ -884,7 +896,9 @@ template <typename T, int DP, int NW, int BQ, bool SINK> void run_dkv(WindowPara
     constexpr bool VLDS = sizeof(T) == 2 && DP >= 96 && !SINK;
     constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK ? 1 : 2;
     p.tiles = tiles;
-    const unsigned grid = xcd_grid(p, p.B * p.Hk * tiles * (SINK ? p.chunks : 1));
+    p.heavy = SINK ? 0 : (p.S > p.key0 ? (p.S - p.key0 + 32 * NW - 1) / (32 * NW) : 0);
+    if (p.heavy >= tiles) p.heavy = 0;                   // nothing but sinks: all alike
+    const unsigned grid = xcd_grid(p, p.B * p.Hk * (tiles - p.heavy) * (SINK ? p.chunks : 1)) + (p.heavy * p.B * p.Hk + 7) / 8 * 8;
     const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * NW * DP * sizeof(T) : 0), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tl > rows ? tl : rows;
     vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), lds);
