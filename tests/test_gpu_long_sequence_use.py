@@ -1,0 +1,142 @@
+"""The long-sequence operators under what a program does around them: saved tensors that were moved to the host and back,
+checkpointing, one tensor in several places, values changed between forward and backward, a single far-strided token, sequences
+near the largest position."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def _block():
+    """A call of every differentiable operator on one projection x [2, 70, 8, 64], and its inputs."""
+    from vit_amd import functional as VF
+    g = _gen(41)
+    x = torch.randn(2, 70, 8, 64, generator=g, device='cuda').bfloat16()
+    gq, gk = (torch.rand(64, generator=g, device='cuda') + 0.5 for _ in range(2))
+    table = VF.rotary_table(torch.arange(70, device='cuda'), 64)
+    pos = torch.randint(0, 70, (2, 70), generator=g, device='cuda')
+    lengths = torch.tensor([70, 33], dtype=torch.int32, device='cuda')
+
+    def run(x, gq, gk):
+        q, k = VF.qk_norm_rotary(x[:, :, :4], x[:, :, 4:6], gq, gk, table, pos=pos)
+        o = VF.window_attention(q, k, x[:, :, 6:], 9, sinks=2, causal=True, lengths=lengths)
+        return VF.rotary(o, table, pos=pos, interleaved=True)
+    do = torch.randn(2, 70, 4, 64, generator=g, device='cuda').bfloat16()
+    return run, (x, gq, gk), do
+
+
+def _grads(run, ins, do):
+    ins = [t.detach().requires_grad_(True) for t in ins]
+    o = run(*ins)
+    junk = [torch.full((2, 70, 8, 64), 9.0, dtype=torch.bfloat16, device='cuda') for _ in range(16)]    # over what was freed
+    grads = torch.autograd.grad(o, ins, do)
+    del junk
+    return (o.detach(), *grads)
+
+
+def test_saved_tensors_moved_to_the_host():
+    run, ins, do = _block()
+    want = _grads(run, ins, do)
+    with torch.autograd.graph.save_on_cpu():
+        got = _grads(run, ins, do)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_checkpointed():
+    from torch.utils.checkpoint import checkpoint
+    run, ins, do = _block()
+    want = _grads(run, ins, do)
+    for reentrant in (False, True):
+        ins2 = [t.detach().requires_grad_(True) for t in ins]
+        o = checkpoint(run, *ins2, use_reentrant=reentrant)
+        o.backward(do)
+        assert all(torch.equal(a, b) for a, b in zip((o.detach(), *(t.grad for t in ins2)), want))
+
+
+def test_one_tensor_as_query_key_and_value():
+    from vit_amd import functional as VF
+    g = _gen(42)
+    x = torch.randn(1, 50, 3, 32, generator=g, device='cuda', requires_grad=True)
+    do = torch.randn(1, 50, 3, 32, generator=g, device='cuda')
+    got, = torch.autograd.grad(VF.window_attention(x, x, x, 5, sinks=1), x, do)
+    parts = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+    dq, dk, dv = torch.autograd.grad(VF.window_attention(*parts, 5, sinks=1), parts, do)
+    # three fp32 values in any order: two roundings of a partial sum
+    assert ((got - (dq + dk + dv)).abs() <= 4 * 2 ** -24 * (dq.abs() + dk.abs() + dv.abs())).all()
+
+
+def test_changed_between_forward_and_backward():
+    from vit_amd import functional as VF
+    run, ins, do = _block()
+    table = VF.rotary_table(torch.arange(70, device='cuda'), 64)
+    lengths = torch.tensor([70, 33], dtype=torch.int32, device='cuda')
+    x = ins[0].detach().requires_grad_(True)
+    for call, what in ((lambda: VF.rotary(x, table), table), (lambda: VF.qk_norm_rotary(x, x, None, None, table)[0], table),
+                       (lambda: VF.window_attention(x, x, x, 4, lengths=lengths), lengths)):
+        o = call()
+        what.mul_(1)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            o.backward(torch.ones_like(o))
+
+
+def test_no_second_derivative():
+    from vit_amd import functional as VF
+    run, ins, do = _block()
+    x = ins[0].detach().requires_grad_(True)
+    table = VF.rotary_table(torch.arange(70, device='cuda'), 64)
+    for call in (lambda: VF.rotary(x, table), lambda: VF.qk_norm_rotary(x, x, None, None, table)[0],
+                 lambda: VF.window_attention(x, x, x, 4)):
+        o = call()
+        dx, = torch.autograd.grad(o, x, torch.ones_like(o), create_graph=True)
+        with pytest.raises(RuntimeError):
+            dx.float().sum().backward()
+
+
+def test_one_token_with_a_far_stride():
+    """The stride of a dimension of one token is nowhere gone along, whatever it is."""
+    from vit_amd import functional as VF
+    x = torch.randn(2, 1, 4, 64, generator=_gen(43), device='cuda').bfloat16()
+    far = torch.as_strided(x, x.shape, (256, 1 << 24, 64, 1))
+    want, got = [], []
+    for src, to in ((x, want), (far, got)):
+        ins = [src.detach().requires_grad_(True) for _ in range(3)]
+        o = VF.window_attention(*ins, 3, causal=True)
+        to += [o.detach(), *torch.autograd.grad(o, ins, src.detach())]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('window,sinks', [(20, 3), (7, 0), (0, 5)])
+def test_decode_near_the_largest_position(window, sinks):
+    """A sequence of 2^31 - 1 tokens sees what a short one sees whose ring stands at the same slot."""
+    from vit_amd import functional as VF
+    g = _gen(44)
+    slots = sinks + window + 3
+    ring = slots - sinks
+    far = 2 ** 31 - 1
+    near = sinks + 4 * ring + (far - sinks) % ring
+    q, k, v = (torch.randn(2, h, 64, generator=g, device='cuda').bfloat16() for h in (4, 2, 2))
+    kc, vc = (torch.randn(2, 2, slots, 64, generator=g, device='cuda').bfloat16() for _ in range(2))
+    res = []
+    for n in (near, far):
+        c = kc.clone(), vc.clone()
+        o = VF.window_decode(q, k, v, *c, torch.full((2,), n, dtype=torch.int32, device='cuda'), window, sinks=sinks)
+        res.append((o, *c))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_prefill_lengths_beyond_the_prompts():
+    """Lengths past the padded width mean the whole width, for the steps after it too."""
+    from vit_amd.window import WindowCache
+    g = _gen(45)
+    x = torch.randn(2, 11, 6, 64, generator=g, device='cuda').bfloat16()
+    t = torch.randn(2, 6, 64, generator=g, device='cuda').bfloat16()
+    res = []
+    for n in ([11, 5], [40, 5]):
+        c = WindowCache(2, 2, 64, 6, 1)
+        o = c.prefill(x[:, :, :2], x[:, :, 2:4], x[:, :, 4:], torch.tensor(n, dtype=torch.int32, device='cuda'))
+        res.append((o, c.step(t[:, :2], t[:, 2:4], t[:, 4:]), c.lengths, c.k, c.v))
+    assert all(torch.equal(a, b) for a, b in zip(*res))

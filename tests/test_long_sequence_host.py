@@ -143,3 +143,11 @@ def test_frequencies():
     for bad in ((63,), (0,), (64, 0.0)):
         with pytest.raises(ValueError):
             rf(*bad)
+
+
+def test_more_work_than_a_launch_holds(L):
+    """Refused by its size, not by a failed launch: workgroups times threads past 2^32."""
+    _bad(L, norm(L, B=1 << 12, N=1 << 16, Hq=1, Hk=1, dh=127, rot=2, rows=1 << 16), 'too many')
+    _bad(L, window(L, B=1 << 24, N=16, Hq=4), 'too many')
+    _bad(L, window(L, B=1 << 14, N=1 << 17, Hk=1, Hq=1), 'too many')
+    _bad(L, decode(L, B=1 << 26), 'too many')

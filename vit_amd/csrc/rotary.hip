@@ -441,8 +441,8 @@ int check_qk_norm(const char* what, int dtype, int B, int N, int Hq, int Hk, int
     VITK_CHECK_ARG(B >= 0 && N >= 0 && Hq >= 1 && Hk >= 1, "%s: bad shape B=%d N=%d Hq=%d Hk=%d", what, B, N, Hq, Hk);
     VITK_CHECK_ARG(dh >= 1 && dh <= 128, "%s: head width %d is outside 1 .. 128", what, dh);
     VITK_CHECK_ARG(eps > 0.f, "%s: eps must be positive", what);
-    VITK_CHECK_ARG((long)B * N * (Hq > Hk ? Hq : Hk) < (1L << 31), "%s: B * N * H = %ld rows are too many", what,
-                   (long)B * N * (Hq > Hk ? Hq : Hk));
+    VITK_CHECK_ARG((long)B * N < (1L << 31) && (long)B * N * ((long)Hq + Hk) < (1L << 31),
+                   "%s: B * N * (Hq + Hk) = %ld rows are too many for one call", what, (long)B * N * ((long)Hq + Hk));
     return VITK_OK;
 }
 unsigned side_blocks(long groups, int lpr_log2, unsigned most) {
@@ -538,6 +538,7 @@ extern "C" int vitk_qk_norm_rotary_fwd(int dtype, int interleaved, int B, int N,
     p.q.y = yq; p.k.y = yk;
     p.q.blocks = side_blocks(p.q.groups, p.lpr_log2, 0);
     p.k.blocks = side_blocks(p.k.groups, p.lpr_log2, 0);
+    VITK_CHECK_ARG((long)p.q.blocks + p.k.blocks < (1L << 24), "%s: too many workgroups for one call", what);      // 2^32 threads
     if (dtype == VITK_BF16) {
         if (V == 8) launch_qk_norm<__bf16, 8, false>(p, interleaved, hpt, stream);
         else if (V == 4) launch_qk_norm<__bf16, 4, false>(p, interleaved, hpt, stream);

@@ -425,7 +425,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     for (int t = 0; t < ND; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) bad += o[t][e] * 0.f;
-    if (__any(!none && bad != 0.f)) {                    // (a NaN is unequal)
+    if ((p.w >= 0 || p.causal) && __any(!none && bad != 0.f && l == l)) {         // (a NaN is unequal; a NaN sum is the row's own)
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -815,6 +815,7 @@ Plan make_plan(int B, int N, int Hq, int Hk, int dh, int w, int S) {
     // their own, whose workgroups share the queries; else they stay in the ordinary one (16 x 577 tokens, window 64: 45 us in
     // all against 33 + 14 + 7).
     pl.sink_keys = w >= 0 && S > 0 && N > 4L * (128 + 2L * w) ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
+    if ((long)B * Hk * pl.sink_keys >= (1L << 22)) pl.sink_keys = 0;     // (their sum would be more than 2^32 threads)
     pl.chunks = pl.per_chunk = 0;
     if (pl.sink_keys) {
         // about 1024 one-wave workgroups, at least 4 query tiles each
@@ -836,6 +837,8 @@ int check_window(const char* what, int dtype, int B, int N, int Hq, int Hk, int 
     VITK_CHECK_ARG(dh >= 8 && dh <= 128 && dh % 8 == 0, "%s: head width %d must be a multiple of 8 up to 128", what, dh);
     VITK_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: the scale must be positive and finite", what);
     VITK_CHECK_ARG(sinks >= 0, "%s: bad number of sinks %d", what, sinks);
+    // two threads a row, at most 2^32 a launch
+    VITK_CHECK_ARG((long)B * Hq * (N + 256L) < (1L << 31), "%s: B * Hq * N = %ld rows are too many for one call", what, (long)B * Hq * N);
     return VITK_OK;
 }
 int check_view(const char* what, const char* name, const View& v, int dtype) {
@@ -862,7 +865,8 @@ unsigned xcd_grid(WindowParams& p, int total) {
     p.total = total;
     p.run = (total + 7) / 8;
     if (p.lengths || (p.causal && p.w < 0)) p.run = total / 32 < 1 ? 1 : (total / 32 > 16 ? 16 : total / 32);
-    return (unsigned)((total + 8 * p.run - 1) / (8 * p.run) * 8 * p.run);
+    const long round = 8L * p.run;
+    return (unsigned)((total + round - 1) / round * round);
 }
 
 template <typename T, int DP, int NW, int BK> void run_fwd(WindowParams p, hipStream_t st) {
@@ -937,6 +941,7 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     if (int e = check_window(what, dtype, B, N, Hq, Hk, dh, scale, sinks)) return e;
     if (B == 0 || N == 0) return VITK_OK;
     WindowParams p = {};
+    if (N == 1) qn = kn = vn = 0;                        // one token: whatever its stride is, nobody goes there
     p.q = View{q, qb, qn, qh};
     p.k = View{k, kb, kn, kh};
     p.v = View{v, vb, vn, vh};
@@ -950,7 +955,6 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     p.o_lo = out_lo;
     p.lse = lse;
     const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
-    VITK_CHECK_ARG((long)B * Hq * ((N + 63) / 64) < (1L << 30), "%s: too many tiles for one call", what);
 #define GO(T, D) if (pl.nwq == 4) run_fwd<T, D, 4>(p, stream); else run_fwd<T, D, 2>(p, stream)
 #define BY_DP(T) switch (pl.dp) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 96: GO(T, 96); break; default: GO(T, 128); break; }
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
@@ -977,10 +981,11 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     if (int e = check_window(what, dtype, B, N, Hq, Hk, dh, scale, sinks)) return e;
     if (B == 0 || N == 0) return VITK_OK;
     WindowParams p = {};
+    if (N == 1) qn = kn = vn = 0;                        // one token: whatever its stride is, nobody goes there
     p.q = View{q, qb, qn, qh};
     p.k = View{k, kb, kn, kh};
     p.v = View{v, vb, vn, vh};
-    p.dout = View{dout, ob, on, oh};
+    p.dout = View{dout, ob, N == 1 ? 0 : on, oh};
     if (int e = check_view(what, "q", p.q, dtype)) return e;
     if (int e = check_view(what, "k", p.k, dtype)) return e;
     if (int e = check_view(what, "v", p.v, dtype)) return e;
@@ -989,7 +994,6 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     VITK_CHECK_ARG(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo) | reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) |
                      reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
                    "%s: out, dq, dk, dv and the workspace must be 16-byte aligned", what);
-    VITK_CHECK_ARG((long)B * Hq * ((N + 63) / 64) < (1L << 30), "%s: too many tiles for one call", what);
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, causal, scale, lengths);
     p.o = out;
     p.o_lo = const_cast<void*>(out_lo);

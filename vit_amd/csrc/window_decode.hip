@@ -111,7 +111,7 @@ struct Seen {
 __device__ __forceinline__ Seen seen_by(const DecodeParams& p, int pos) {
     Seen s;
     s.lost = p.w < 0 && pos >= p.C;
-    s.n1 = pos < 0 || s.lost || p.w < 0 ? 0 : min(p.S, pos + 1);
+    s.n1 = pos < 0 || s.lost || p.w < 0 ? 0 : (pos < p.S ? pos + 1 : p.S);
     const int lo = p.w < 0 ? 0 : max(p.S, pos - p.w);
     s.n = pos < 0 || s.lost ? 0 : s.n1 + max(0, pos - lo + 1);
     s.R = p.w < 0 ? p.C : p.C - p.S;
@@ -564,7 +564,7 @@ extern "C" int vitk_window_decode(int dtype, int B, int Hq, int Hk, int dh, cons
     p.splits = d.splits; p.gblocks = d.gblocks; p.keys_per_split = d.per;
     VITK_CHECK_ARG(d.splits == 1 || workspace, "%s: this shape needs a workspace", what);
     const long blocks = (long)B * Hk * d.gblocks * d.splits;
-    VITK_CHECK_ARG(blocks < (1L << 31), "%s: too many workgroups for one call", what);
+    VITK_CHECK_ARG(blocks * d.nw * 64 < (1L << 32) && (long)B * Hq * 128 < (1L << 32), "%s: too many workgroups for one call", what);
     const int chunks = dh * es / 16;                      // lanes a key's row takes, up to a power of two
     if (dtype == VITK_BF16) {
         if (chunks <= 4) decode_heads<__bf16, 4>(p, d, blocks, stream);

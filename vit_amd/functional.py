@@ -1121,13 +1121,12 @@ class RotaryFn(torch.autograd.Function):
         x = _unit_heads(x)
         ctx.plan = ops.rotary_plan(x, table, pos, offset, interleaved)
         ctx.save_for_backward(table, pos)
-        return ops.rotary_run(ctx.plan, x, 0)
+        return ops.rotary_run(ctx.plan, x, table, pos, 0)
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        ctx.saved_tensors                # alive, and unchanged since
-        return ops.rotary_run(ctx.plan, _unit_heads(dy), 1), None, None, None, None
+        return ops.rotary_run(ctx.plan, _unit_heads(dy), *ctx.saved_tensors, 1), None, None, None, None
 
 
 def rotary(x, table, pos=None, offset=0, interleaved=False):
@@ -1143,14 +1142,13 @@ class QkNormRotaryFn(torch.autograd.Function):
         q, k = _unit_heads(q), _unit_heads(k)
         ctx.plan = ops.qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
         ctx.save_for_backward(q, k, gamma_q, gamma_k, table, pos)
-        return ops.qk_norm_rotary_fwd(ctx.plan, q, k)
+        return ops.qk_norm_rotary_fwd(ctx.plan, q, k, gamma_q, gamma_k, table, pos)
 
     @staticmethod
     @_once
     def backward(ctx, dq, dk):
-        ctx.saved_tensors                # alive, and unchanged since
         want = ctx.needs_input_grad
-        grads = ops.qk_norm_rotary_bwd(ctx.plan, _unit_heads(dq), _unit_heads(dk), want[2], want[3])
+        grads = ops.qk_norm_rotary_bwd(ctx.plan, *ctx.saved_tensors, _unit_heads(dq), _unit_heads(dk), want[2], want[3])
         return (*grads, None, None, None, None, None)
 
 
@@ -1167,17 +1165,16 @@ class WindowAttentionFn(torch.autograd.Function):
         q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
         plan = ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths)
         train = any(ctx.needs_input_grad[:3])
-        out, lse, lo = ops.window_attn_fwd(plan, q, train)
+        out, lse, lo = ops.window_attn_fwd(plan, q, k, v, lengths, train)
         if train:
             ctx.plan, ctx.ws_bytes = plan, ops.window_attn_bwd_workspace(plan)
-            ctx.save_for_backward(q, k, v, out, lse, lo, lengths)
+            ctx.save_for_backward(q, k, v, lengths, out, lse, lo)
         return out
 
     @staticmethod
     @_once
     def backward(ctx, dout):
-        _, _, _, out, lse, lo, _ = ctx.saved_tensors
-        return (*ops.window_attn_bwd(ctx.plan, ctx.ws_bytes, out, lse, lo, ops._aligned_heads(dout)), None, None, None, None, None)
+        return (*ops.window_attn_bwd(ctx.plan, ctx.ws_bytes, *ctx.saved_tensors, ops._aligned_heads(dout)), None, None, None, None, None)
 
 
 def window_attention(q, k, v, window, sinks=0, causal=False, scale=None, lengths=None):

@@ -570,48 +570,59 @@ def rotary_table(positions, freqs, mul=1.0):
     return table
 
 
-def _turn_args(what, B, N, dh, table, pos, offset):
-    """(table pointer, rows, rotated width, ids pointer, ids are int64, offset) of a call over [B, N] tokens."""
+def _check_turn(what, B, N, dh, table, pos, offset):
+    """Checks the positions of a call over [B, N] tokens; the offset."""
     if table is None:
         if pos is not None or offset:
             raise ValueError(f'{what}: positions without a table')
-        return 0, 0, 0, 0, 0, 0
+        return 0
     if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous():
         raise ValueError(f'{what}: the table must be contiguous fp32 [rows, pairs, 2] (rotary_table)')
     if 2 * table.shape[1] > dh:
         raise ValueError(f'{what}: the table turns {2 * table.shape[1]} elements of heads of {dh}')
     if pos is None:
-        return table.data_ptr(), table.shape[0], 2 * table.shape[1], 0, 0, int(offset)
+        return int(offset)
     if offset:
         raise ValueError(f'{what}: give pos or offset, not both')
     if tuple(pos.shape) != (B, N) or pos.dtype not in (torch.int32, torch.int64) or not pos.is_contiguous():
         raise ValueError(f'{what}: pos must be contiguous int32 / int64 [B, N]')
-    return table.data_ptr(), table.shape[0], 2 * table.shape[1], pos.data_ptr(), int(pos.dtype == torch.int64), 0
+    return 0
 
 
-# The autograd Functions check a call once, in the forward (*_plan: sizes, types, pointers of what is kept for the backward),
-# and run it twice: the backward's Python runs in autograd's own thread, where every line of it costs several times more.
+def _turn_args(table, pos, offset):
+    """(table pointer, rows, rotated width, ids pointer, ids are int64, offset)"""
+    if table is None:
+        return 0, 0, 0, 0, 0, 0
+    rows, pairs, _ = table.shape
+    if pos is None:
+        return table.data_ptr(), rows, 2 * pairs, 0, 0, offset
+    return table.data_ptr(), rows, 2 * pairs, pos.data_ptr(), int(pos.dtype == torch.int64), 0
+
+
+# The autograd Functions check a call once, in the forward (*_plan: sizes, types, the device), and run it twice (*_fwd, *_bwd:
+# pointers and strides of the tensors at hand, which need not be the forward's own where saved tensors were offloaded or made
+# again): the backward's Python runs in autograd's own thread, where every line of it costs several times more.
 def rotary_plan(x, table, pos, offset, interleaved):
     dev = _req_here(x, table, pos)
     (B, N, H, dh), _ = _heads(x, 'rotary x')
     if table is None:
         raise ValueError('rotary: no table')
-    return _dt(x), int(interleaved), B, N, H, dh, _turn_args('rotary', B, N, dh, table, pos, offset), dev
+    return _dt(x), int(interleaved), B, N, H, dh, _check_turn('rotary', B, N, dh, table, pos, offset), dev
 
 
-def rotary_run(plan, x, inverse):
-    dt, inter, B, N, H, dh, turn, dev = plan
+def rotary_run(plan, x, table, pos, inverse):
+    dt, inter, B, N, H, dh, offset, dev = plan
     sb, sn, sh, _ = x.stride()
     y = x.new_empty((B, N, H, dh))
-    check(lib().vitk_rotary(dt, inverse, inter, B, N, H, dh, x.data_ptr(), sb, sn, sh, *turn, y.data_ptr(), _stream_on(dev)),
-          'vitk_rotary')
+    check(lib().vitk_rotary(dt, inverse, inter, B, N, H, dh, x.data_ptr(), sb, sn, sh, *_turn_args(table, pos, offset), y.data_ptr(),
+                            _stream_on(dev)), 'vitk_rotary')
     return y
 
 
 def rotary(x, table, pos=None, offset=0, interleaved=False, inverse=False):
     """Rotary positions on x [B, N, H, dh] (any strides, contiguous heads): a new contiguous tensor.  Token (b, n) takes table row
     pos[b, n], or offset + n; ids outside the table give NaN.  ``inverse``: the adjoint."""
-    return rotary_run(rotary_plan(x, table, pos, offset, interleaved), x, int(inverse))
+    return rotary_run(rotary_plan(x, table, pos, offset, interleaved), x, table, pos, int(inverse))
 
 
 def _check_qk(q, k, gamma_q, gamma_k):
@@ -627,23 +638,28 @@ def _check_qk(q, k, gamma_q, gamma_k):
 
 def qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved):
     dev = _req_here(q, k, gamma_q, gamma_k, table, pos)
-    B, N, Hq, Hk, dh, sq, sk = _check_qk(q, k, gamma_q, gamma_k)
-    turn = _turn_args('qk_norm_rotary', B, N, dh, table, pos, offset)
-    return ((_dt(q), int(interleaved), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2],
-             _ptr(gamma_q), _ptr(gamma_k), float(eps), *turn), dev)
+    B, N, Hq, Hk, dh, _, _ = _check_qk(q, k, gamma_q, gamma_k)
+    offset = _check_turn('qk_norm_rotary', B, N, dh, table, pos, offset)
+    return (_dt(q), int(interleaved), B, N, Hq, Hk, dh), float(eps), offset, dev
 
 
-def qk_norm_rotary_fwd(plan, q, k):
-    args, dev = plan
+def _qk_args(plan, q, k, gamma_q, gamma_k, table, pos):
+    sizes, eps, offset, _ = plan
+    s, r = q.stride(), k.stride()
+    return (*sizes, q.data_ptr(), s[0], s[1], s[2], k.data_ptr(), r[0], r[1], r[2], _ptr(gamma_q), _ptr(gamma_k), eps,
+            *_turn_args(table, pos, offset))
+
+
+def qk_norm_rotary_fwd(plan, q, k, gamma_q, gamma_k, table, pos):
     yq, yk = q.new_empty(q.shape), k.new_empty(k.shape)
-    check(lib().vitk_qk_norm_rotary_fwd(*args, yq.data_ptr(), yk.data_ptr(), _stream_on(dev)), 'vitk_qk_norm_rotary_fwd')
+    check(lib().vitk_qk_norm_rotary_fwd(*_qk_args(plan, q, k, gamma_q, gamma_k, table, pos), yq.data_ptr(), yk.data_ptr(),
+                                        _stream_on(plan[3])), 'vitk_qk_norm_rotary_fwd')
     return yq, yk
 
 
-def qk_norm_rotary_bwd(plan, dyq, dyk, want_dgq, want_dgk):
+def qk_norm_rotary_bwd(plan, q, k, gamma_q, gamma_k, table, pos, dyq, dyk, want_dgq, want_dgk):
     """(dq, dk, dgamma_q, dgamma_k); a gamma gradient that is not wanted is None."""
-    args, dev = plan
-    dh = args[6]
+    dh = plan[0][6]
     dq, dk = dyq.new_empty(dyq.shape), dyk.new_empty(dyk.shape)
     dgq = dgk = ws = None
     if want_dgq or want_dgk:
@@ -651,8 +667,9 @@ def qk_norm_rotary_bwd(plan, dyq, dyk, want_dgq, want_dgk):
         dgq, dgk = dg[0] if want_dgq else None, dg[1] if want_dgk else None
         ws = dyq.new_empty(lib().vitk_qk_norm_rotary_bwd_workspace_bytes(dh), dtype=torch.uint8)
     s, r = dyq.stride(), dyk.stride()
-    check(lib().vitk_qk_norm_rotary_bwd(*args, dyq.data_ptr(), s[0], s[1], s[2], dyk.data_ptr(), r[0], r[1], r[2], dq.data_ptr(),
-                                        dk.data_ptr(), _ptr(dgq), _ptr(dgk), _ptr(ws), _stream_on(dev)), 'vitk_qk_norm_rotary_bwd')
+    check(lib().vitk_qk_norm_rotary_bwd(*_qk_args(plan, q, k, gamma_q, gamma_k, table, pos), dyq.data_ptr(), s[0], s[1], s[2],
+                                        dyk.data_ptr(), r[0], r[1], r[2], dq.data_ptr(), dk.data_ptr(), _ptr(dgq), _ptr(dgk), _ptr(ws),
+                                        _stream_on(plan[3])), 'vitk_qk_norm_rotary_bwd')
     return dq, dk, dgq, dgk
 
 
@@ -680,40 +697,45 @@ def _i32(n):
 
 
 def window_attn_plan(q, k, v, window, sinks, causal, scale, lengths):
-    """q, k, v with 16-byte aligned rows (_aligned_heads)."""
     dev = _req_here(q, k, v, lengths)
-    B, N, Hq, Hk, dh, sq, sk, sv = _check_window(q, k, v, window, sinks, lengths)
-    return ((_dt(q), B, N, Hq, Hk, dh, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0],
-             sv[1], sv[2], float(scale), _i32(window), _i32(sinks), int(causal), _ptr(lengths)), dev)
+    B, N, Hq, Hk, dh, _, _, _ = _check_window(q, k, v, window, sinks, lengths)
+    return (_dt(q), B, N, Hq, Hk, dh), (float(scale), _i32(window), _i32(sinks), int(causal)), dev
 
 
-def window_attn_fwd(plan, q, train=True):
+def _window_args(plan, q, k, v, lengths):
+    """q, k, v with 16-byte aligned rows (_aligned_heads)."""
+    sizes, rule, _ = plan
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
+    return (*sizes, q.data_ptr(), sq[0], sq[1], sq[2], k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2], *rule,
+            _ptr(lengths))
+
+
+def window_attn_fwd(plan, q, k, v, lengths, train=True):
     """(out [B, N, Hq, dh], lse [B, Hq, N] in log2, out_lo): lse and, in bf16, what out's rounding took (out_lo) are for the
     backward, None without ``train``."""
-    args, dev = plan
-    B, N, Hq = args[1:4]
+    dt, B, N, Hq, _, _ = plan[0]
     out = q.new_empty(q.shape)
     lse = q.new_empty((B, Hq, N), dtype=torch.float32) if train else None
-    lo = q.new_empty(q.shape) if train and args[0] == BF16 else None
-    check(lib().vitk_window_attn_fwd(*args, out.data_ptr(), _ptr(lo), _ptr(lse), _stream_on(dev)), 'vitk_window_attn_fwd')
+    lo = q.new_empty(q.shape) if train and dt == BF16 else None
+    check(lib().vitk_window_attn_fwd(*_window_args(plan, q, k, v, lengths), out.data_ptr(), _ptr(lo), _ptr(lse), _stream_on(plan[2])),
+          'vitk_window_attn_fwd')
     return out, lse, lo
 
 
 def window_attn_bwd_workspace(plan):
     """Bytes that window_attn_bwd needs beside its results."""
-    a = plan[0]
-    return lib().vitk_window_attn_bwd_workspace_bytes(*a[:6], a[19], a[20])
+    return lib().vitk_window_attn_bwd_workspace_bytes(*plan[0], plan[1][1], plan[1][2])
 
 
-def window_attn_bwd(plan, ws_bytes, out, lse, lo, dout):
+def window_attn_bwd(plan, ws_bytes, q, k, v, lengths, out, lse, lo, dout):
     """(dq, dk, dv), contiguous."""
-    args, dev = plan
-    B, N, Hq, Hk, dh = args[1:6]
+    _, B, N, Hq, Hk, dh = plan[0]
     dq, dk, dv = dout.new_empty((B, N, Hq, dh)), dout.new_empty((B, N, Hk, dh)), dout.new_empty((B, N, Hk, dh))
     ws = dout.new_empty(ws_bytes, dtype=torch.uint8)
     s = dout.stride()
-    check(lib().vitk_window_attn_bwd(*args, out.data_ptr(), _ptr(lo), lse.data_ptr(), dout.data_ptr(), s[0], s[1], s[2], dq.data_ptr(),
-                                     dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), _stream_on(dev)), 'vitk_window_attn_bwd')
+    check(lib().vitk_window_attn_bwd(*_window_args(plan, q, k, v, lengths), out.data_ptr(), _ptr(lo), lse.data_ptr(), dout.data_ptr(),
+                                     s[0], s[1], s[2], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(),
+                                     _stream_on(plan[2])), 'vitk_window_attn_bwd')
     return dq, dk, dv
 
 

@@ -275,7 +275,8 @@ rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
 def qk_norm_rotary(q: Tensor, k: Tensor, gamma_q: Optional[Tensor], gamma_k: Optional[Tensor], table: Optional[Tensor],
                    pos: Optional[Tensor], offset: int, eps: float, interleaved: bool) -> Tuple[Tensor, Tensor]:
     q, k = _unit(q), _unit(k)
-    return ops.qk_norm_rotary_fwd(ops.qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved), q, k)
+    plan = ops.qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
+    return ops.qk_norm_rotary_fwd(plan, q, k, gamma_q, gamma_k, table, pos)
 
 
 @qk_norm_rotary.register_fake
@@ -289,7 +290,7 @@ def qk_norm_rotary_backward(dyq: Tensor, dyk: Tensor, q: Tensor, k: Tensor, gamm
                             interleaved: bool) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     q, k = _unit(q), _unit(k)
     plan = ops.qk_norm_rotary_plan(q, k, gamma_q, gamma_k, table, pos, offset, eps, interleaved)
-    dq, dk, dgq, dgk = ops.qk_norm_rotary_bwd(plan, _unit(dyq), _unit(dyk), True, True)
+    dq, dk, dgq, dgk = ops.qk_norm_rotary_bwd(plan, q, k, gamma_q, gamma_k, table, pos, _unit(dyq), _unit(dyk), True, True)
     return dq, dk, dgq.clone(), dgk.clone()                  # custom-op outputs may not alias each other
 
 
@@ -318,7 +319,7 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, c
                      lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
     """out_lo: what bf16's rounding took from out, for the backward (empty in fp32)."""
     q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
-    out, lse, lo = ops.window_attn_fwd(ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths), q)
+    out, lse, lo = ops.window_attn_fwd(ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths), q, k, v, lengths)
     return out, lse, q.new_empty(0) if lo is None else lo
 
 
@@ -334,8 +335,8 @@ def window_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out
                               lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
     q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
     plan = ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths)
-    return ops.window_attn_bwd(plan, ops.window_attn_bwd_workspace(plan), out, lse, out_lo if out_lo.numel() else None,
-                               ops._aligned_heads(dout))
+    return ops.window_attn_bwd(plan, ops.window_attn_bwd_workspace(plan), q, k, v, lengths, out, lse,
+                               out_lo if out_lo.numel() else None, ops._aligned_heads(dout))
 
 
 @window_attention_backward.register_fake

@@ -41,7 +41,7 @@ class WindowCache:
         if lengths is None:
             self.lengths.fill_(k.shape[1])
         else:
-            self.lengths.copy_(lengths)
+            self.lengths.copy_(lengths.clamp(max=k.shape[1]))
         return out
 
     @torch.no_grad()
