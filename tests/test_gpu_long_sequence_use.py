@@ -4,6 +4,8 @@ near the largest position."""
 import pytest
 import torch
 
+import long_ref as R
+
 pytestmark = pytest.mark.gpu
 
 
@@ -140,3 +142,21 @@ def test_prefill_lengths_beyond_the_prompts():
         o = c.prefill(x[:, :, :2], x[:, :, 2:4], x[:, :, 4:], torch.tensor(n, dtype=torch.int32, device='cuda'))
         res.append((o, c.step(t[:, :2], t[:, 2:4], t[:, 4:]), c.lengths, c.k, c.v))
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.parametrize('case', [(1, 87, 2, 1, 128, 2, 1, True), (2, 40, 3, 3, 64, -1, 0, False), (1, 200, 2, 2, 40, 90, 3, True),
+                                  (1, 700, 2, 1, 96, 3, 2, True), (1, 5, 1, 1, 64, 1, 0, False)], ids=str)
+def test_small_calls_round_once(monkeypatch, case):
+    """Where a call has few scores, P, dS and o in D are held as two bf16 each (a rounding's remainder is under 2^-8 of the value,
+    and is rounded by 2^-8 of itself): 2^-16 where large calls have 2^-8, and then the result's own rounding."""
+    from vit_amd import functional as VF
+    B, N, Hq, Hk, dh, window, sinks, causal = case
+    g = _gen(46)
+    q, k, v, do = (torch.randn(B, N, h, dh, generator=g, device='cuda').bfloat16() for h in (Hq, Hk, Hk, Hq))
+    ins = [t.requires_grad_(True) for t in (q, k, v)]
+    o = VF.window_attention(*ins, window, sinks=sinks, causal=causal)
+    got = dict(zip(('o', 'dq', 'dk', 'dv'), (o.detach(), *torch.autograd.grad(o, ins, do))))
+    monkeypatch.setattr(R, 'unit', lambda dtype: 2.0 ** -16)
+    want = R.window_attention(*(t.detach() for t in ins), window, sinks, causal, dh ** -0.5, None, do)
+    for t, x in got.items():
+        R.within(x, want[t][0], want[t][1] + 2.0 ** -8 * want[t][0].abs(), t)

@@ -34,6 +34,11 @@ template <typename T> __device__ __forceinline__ void acc_frag(Frag<T>& f, const
 #pragma unroll
     for (int e = 0; e < 8; ++e) frag_set_f(f, e, a[8 * s + e]);
 }
+// what the rounding to acc_frag's bf16 took
+__device__ __forceinline__ void rest_frag(Frag<__bf16>& r, const Frag<__bf16>& f, const f32x16& a, int s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) frag_set_f(r, e, a[8 * s + e] - frag_get_f(f, e));
+}
 // LDS image of a tile: rows of CPR 16-byte chunks without padding (what the asynchronous loads can write: 64 consecutive
 // chunks an instruction); chunk c of row r sits at place c ^ swz(r).  The 64 banks hold 16 chunks.  A row fragment reads
 // one chunk of each row: over 16 rows swz (with the row's own offset where a row is shorter than the banks) takes every
@@ -293,7 +298,7 @@ __device__ __forceinline__ void hide(f32x16 (&s)[NS], int kind, const RowRange& 
 }
 
 // ---------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DP, int NW, int BK, int WPE>
+template <typename T, int DP, int NW, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
@@ -405,13 +410,15 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
             for (int u = 0; u < NS; ++u)
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
-                    Frag<T> pf;
+                    Frag<T> pf, rest;
                     acc_frag(pf, s[u], ks);
+                    if constexpr (FINE) rest_frag(rest, pf, s[u], ks);
 #pragma unroll
                     for (int t = 0; t < ND; ++t) {
                         Frag<T> a;
                         col_frag32<DP>(a, Vs, 32 * u + 16 * ks, 32 * t, lane);
                         o[t] = mma32(a, pf, o[t]);
+                        if constexpr (FINE) o[t] = mma32(a, rest, o[t]);
                     }
                 }
         }
@@ -471,7 +478,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
 }
 
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
-template <typename T, int DP, int NW, int BK, int WPE>
+template <typename T, int DP, int NW, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
     constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
@@ -567,13 +574,15 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
                 }
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
-                    Frag<T> sf;
+                    Frag<T> sf, rest;
                     acc_frag(sf, s, ks);
+                    if constexpr (FINE) rest_frag(rest, sf, s, ks);
 #pragma unroll
                     for (int t = 0; t < ND; ++t) {
                         Frag<T> a;
                         col_frag32<DP>(a, Ks, 32 * u + 16 * ks, 32 * t, lane);
                         dq[t] = mma32(a, sf, dq[t]);
+                        if constexpr (FINE) dq[t] = mma32(a, rest, dq[t]);
                     }
                 }
             }
@@ -588,7 +597,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
 // every head of the group.  SINK: one wave, the 32 keys of a sinks' tile and a share of ALL the query tiles, fp32 partial
 // sums out (window_sink_sum_kernel adds the shares in order).
-template <typename T, int DP, int NW, int BQ, bool SINK, bool VLDS, int WPE>
+template <typename T, int DP, int NW, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
     constexpr int NT = 64 * NW, NS = BQ / 32, KD = DP / 16, ND = DP / 32, TILE = BQ * DP;
@@ -714,16 +723,22 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            Frag<T> pf, sf;
+            Frag<T> pf, sf, pr, sr;
             acc_frag(pf, s, ks);
             acc_frag(sf, dp, ks);
+            if constexpr (FINE) {
+                rest_frag(pr, pf, s, ks);
+                rest_frag(sr, sf, dp, ks);
+            }
 #pragma unroll
             for (int t = 0; t < ND; ++t) {
                 Frag<T> a;
                 col_frag32<DP>(a, Ds, 32 * u + 16 * ks, 32 * t, lane);
                 dv[t] = mma32(a, pf, dv[t]);
+                if constexpr (FINE) dv[t] = mma32(a, pr, dv[t]);
                 col_frag32<DP>(a, Qs, 32 * u + 16 * ks, 32 * t, lane);
                 dk[t] = mma32(a, sf, dk[t]);
+                if constexpr (FINE) dk[t] = mma32(a, sr, dk[t]);
             }
         }
     };
@@ -799,16 +814,25 @@ struct Plan {                  // tiles of one call
     int nwq, nwk;              // waves of a query / key workgroup
     int sink_keys;             // keys that the sinks' launch takes (a multiple of 32, 0: none)
     int chunks, per_chunk;
+    bool fine;                 // bf16: P and dS as two bf16 each
 };
+constexpr long FINE = 1 << 17;
 constexpr int SINK_BQ = 32;
-constexpr int NARROW = 128;
+constexpr int NARROW = 256;
 
 // Fewer, larger workgroups read K and V fewer times; they are halved where the large ones would leave CUs without work.
 int waves_for(long rows_tiles_of_128) { return rows_tiles_of_128 >= 512 ? 4 : 2; }
 
-Plan make_plan(int B, int N, int Hq, int Hk, int dh, int w, int S) {
+Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S) {
     Plan pl;
     pl.dp = (dh + 31) / 32 * 32;
+    // P and dS are rounded to bf16 for their products, an error of the size of the results' own rounding as long as many share in
+    // it.  In a call of few scores single ones can carry dq and dk (up to 87 tokens, window 2: 0.0021 of the norm before the
+    // result's own rounding, 0.0017 in large calls): there what the rounding took is multiplied too, in the forward as well,
+    // whose error dq and dk have through o . do (256 tokens x 4 heads of 64: forward 9.4 us against 8.6, backward 23.9 against
+    // 21.5).
+    const long keys = w < 0 ? N : (2L * w + 1 + S < N ? 2L * w + 1 + S : N);
+    pl.fine = dtype == VITK_BF16 && (long)B * Hq * N * keys <= FINE;
     pl.nwq = waves_for((long)B * Hq * ((N + 127) / 128));
     pl.nwk = waves_for((long)B * Hk * ((N + 127) / 128));
     // The sinks' keys are seen by all N queries, other keys by 2 w + 1: where that is over four times more, they get a launch of
@@ -869,56 +893,60 @@ unsigned xcd_grid(WindowParams& p, int total) {
     return (unsigned)((total + round - 1) / round * round);
 }
 
-template <typename T, int DP, int NW, int BK> void run_fwd(WindowParams p, hipStream_t st) {
+template <typename T, int DP, int NW, int BK, bool FINE = false> void run_fwd_tiles(WindowParams p, hipStream_t st) {
     constexpr int WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;           // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK, WPE>), lds);
-    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK, WPE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
-// Key tiles of 64 in bf16; of 32 where the window is narrow and a tile of 64 would be mostly edge (16 x 577 tokens x 12 heads
-// of 64: window 64 on both sides 22.6 us against 26.5; causal window of 512 55 against 53, of 1024 222 against 190).
-template <typename T, int DP, int NW> void run_fwd(const WindowParams& p, hipStream_t st) {
+// Key tiles of 64 in bf16; of 32 where the window is narrow and a tile of 64 would be mostly edge (16 x 577 tokens x 12 heads of
+// 64, window 64 on both sides: 24.1 us against 27.1, window 256: 33.5 against 34.7; 2 x 8192 x 16 heads of 128, causal window
+// of 512: 124.4 against 123.0, 16384 x 16, of 1024: 222 against 190).
+template <typename T, int DP> void run_fwd(const WindowParams& p, const Plan& pl, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        if (p.w < 0 || p.w > NARROW) return run_fwd<T, DP, NW, 64>(p, st);
+        const bool narrow = p.w >= 0 && p.w <= NARROW;
+        if (pl.fine) return narrow ? run_fwd_tiles<T, DP, 2, 32, true>(p, st) : run_fwd_tiles<T, DP, 2, 64, true>(p, st);
+        if (!narrow) return pl.nwq == 4 ? run_fwd_tiles<T, DP, 4, 64>(p, st) : run_fwd_tiles<T, DP, 2, 64>(p, st);
     }
-    run_fwd<T, DP, NW, 32>(p, st);
+    if (pl.nwq == 4) run_fwd_tiles<T, DP, 4, 32>(p, st);
+    else run_fwd_tiles<T, DP, 2, 32>(p, st);
 }
-template <typename T, int DP, int NW> void run_dq(WindowParams p, hipStream_t st) {
+template <typename T, int DP, int NW, bool FINE = false> void run_dq(WindowParams p, hipStream_t st) {
     constexpr int BK = 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;
     p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
     const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tiles > rows ? tiles : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK, WPE>), lds);
-    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK, WPE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
-template <typename T, int DP, int NW, int BQ, bool SINK> void run_dkv(WindowParams p, int tiles, hipStream_t st) {
+template <typename T, int DP, int NW, int BQ, bool SINK, bool FINE = false> void run_dkv(WindowParams p, int tiles, hipStream_t st) {
     // V rows in LDS where they, K's and both accumulators do not fit the registers of two waves a SIMD
     constexpr bool VLDS = sizeof(T) == 2 && DP >= 96 && !SINK;
-    constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK ? 1 : 2;
+    constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK || (FINE && DP == 128) ? 1 : 2;
     p.tiles = tiles;
     p.heavy = SINK ? 0 : (p.S > p.key0 ? (p.S - p.key0 + 32 * NW - 1) / (32 * NW) : 0);
     if (p.heavy >= tiles) p.heavy = 0;                   // nothing but sinks: all alike
     const unsigned grid = xcd_grid(p, p.B * p.Hk * (tiles - p.heavy) * (SINK ? p.chunks : 1)) + (p.heavy * p.B * p.Hk + 7) / 8 * 8;
     const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * NW * DP * sizeof(T) : 0), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
     const size_t lds = tl > rows ? tl : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), lds);
-    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
-template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
+template <typename T, int DP, bool FINE> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
     constexpr int BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     p.out = dq;
-    if (pl.nwq == 4) run_dq<T, DP, 4>(p, st);
-    else run_dq<T, DP, 2>(p, st);
+    if (!FINE && pl.nwq == 4) run_dq<T, DP, 4>(p, st);
+    else run_dq<T, DP, 2, FINE>(p, st);
     if (pl.sink_keys) {
         WindowParams s = p;
         s.key0 = 0;
         s.chunks = pl.chunks;
         s.per_chunk = pl.per_chunk;
-        run_dkv<T, DP, 1, SINK_BQ, true>(s, pl.sink_keys / 32, st);
+        run_dkv<T, DP, 1, SINK_BQ, true, FINE>(s, pl.sink_keys / 32, st);
         s.tiles = pl.sink_keys / 32;
         hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles * 2 * (DP / 2))), dim3(256),
                            0, st, s);
@@ -926,9 +954,15 @@ template <typename T, int DP> void run_bwd(WindowParams p, const Plan& pl, void*
     p.key0 = pl.sink_keys;
     const int rest = p.N - pl.sink_keys;
     if (rest > 0) {
-        if (pl.nwk == 4) run_dkv<T, DP, 4, BQ, false>(p, (rest + 127) / 128, st);
-        else run_dkv<T, DP, 2, BQ, false>(p, (rest + 63) / 64, st);
+        if (!FINE && pl.nwk == 4) run_dkv<T, DP, 4, BQ, false>(p, (rest + 127) / 128, st);
+        else run_dkv<T, DP, 2, BQ, false, FINE>(p, (rest + 63) / 64, st);
     }
+}
+template <typename T, int DP> void run_bwd(const WindowParams& p, const Plan& pl, void* dq, hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (pl.fine) return run_bwd<T, DP, true>(p, pl, dq, st);
+    }
+    run_bwd<T, DP, false>(p, pl, dq, st);
 }
 
 }  // namespace
@@ -954,8 +988,8 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     p.out = out;
     p.o_lo = out_lo;
     p.lse = lse;
-    const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
-#define GO(T, D) if (pl.nwq == 4) run_fwd<T, D, 4>(p, stream); else run_fwd<T, D, 2>(p, stream)
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+#define GO(T, D) run_fwd<T, D>(p, pl, stream)
 #define BY_DP(T) switch (pl.dp) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 96: GO(T, 96); break; default: GO(T, 128); break; }
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
     else { BY_DP(float) }
@@ -968,7 +1002,7 @@ extern "C" long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, in
     if (B <= 0 || N <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || dh < 8 || dh > 128 || sinks < 0) return 0;
     WindowParams p = {};
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, 0, 1.f, nullptr);
-    const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
     return ((long)B * Hq * N + 3) / 4 * 16 + part_floats(pl, B, Hk) * 4;
 }
 
@@ -1002,7 +1036,7 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     p.part = p.delta + ((long)B * Hq * N + 3) / 4 * 4;
     p.dk = dk;
     p.dv = dv;
-    const Plan pl = make_plan(B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
 #define GO(T, D) run_bwd<T, D>(p, pl, dq, stream)
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
     else { BY_DP(float) }
