@@ -12,6 +12,7 @@
 // V tile in LDS by transpose reads in that same order).  Nothing of size N x N exists and nothing is summed by atomics:
 // the backward makes the scores twice (queries' kernel, keys' kernel).  Sums, maxima and the softmax are fp32; with bf16
 // inputs P and dS are rounded to bf16 as operands of their MFMA, each once.
+#include <algorithm>
 #include "common.h"
 
 namespace vitk {
@@ -297,11 +298,27 @@ __device__ __forceinline__ void hide(f32x16 (&s)[NS], int kind, const RowRange& 
 #undef VITK_HIDE
 }
 
+// Accumulators of the wave that had the other half of the keys (or queries), through LDS: at [register][lane].  Two barriers
+// around the pair: put by one, added by the other.
+template <int ND> __device__ __forceinline__ void half_put(float* x, const f32x16 (&a)[ND], int lane) {
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[(16 * t + e) * 64 + lane] = a[t][e];
+}
+template <int ND> __device__ __forceinline__ void half_add(const float* x, f32x16 (&a)[ND], float mine, float other, int lane) {
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) a[t][e] = a[t][e] * mine + x[(16 * t + e) * 64 + lane] * other;
+}
+
 // ---------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DP, int NW, int BK, int WPE, bool FINE>
+// A wave owns 32 queries; KS = 2: two waves share them, each with one half of every tile of keys.
+template <typename T, int DP, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
+    constexpr int NT = 64 * NW, RG = NW / KS, NS = BK / 32 / KS, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (K tile, V tile)
     const int id = xcd_order((int)blockIdx.x, p.total, p.run);
@@ -311,7 +328,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     const int r1 = uniform(id / p.G), g = id - r1 * p.G;
     const int bh = uniform(r1 / p.tiles), tq = r1 - bh * p.tiles;
     const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk, h = hk * p.G + g;
-    const int i0 = 32 * NW * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * wave;
+    const int part = KS == 1 ? 0 : uniform(wave / RG), rg = wave - part * RG;
+    const int i0 = 32 * RG * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * rg;
     const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
     const int i = iw + (lane & 31);
 
@@ -320,7 +338,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     Frag<T> qf[KD];
     own_rows<T, DP>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
 
-    const KeyTiles kt = key_tiles(p, i0, i0 + 32 * NW, len, BK);
+    const KeyTiles kt = key_tiles(p, i0, i0 + 32 * RG, len, BK);
     const RowRange rr = row_range(p, i, len);
     f32x16 o[ND];
 #pragma unroll
@@ -340,7 +358,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
         sv.load(V, p.v.sn, j0, len, p.dh, lds + TILE, wave);
     }
     for (int it = 0; it < kt.n; ++it) {
-        const T* Ks = lds + (it & 1) * 2 * TILE;
+        const T* Ks = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
         const T* Vs = Ks + TILE;
         tile_ready();                                    // and the other buffer's readers are done
         if (it + 1 < kt.n) {
@@ -349,8 +367,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
             sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
             sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
         }
-        const int j0 = BK * key_tile(kt, it);
-        const int kind = tile_kind(p, iw, 32, j0, BK, len);  // the same for the whole wave
+        const int j0 = BK * key_tile(kt, it) + 32 * NS * part;
+        const int kind = tile_kind(p, iw, 32, j0, 32 * NS, len);         // the same for the whole wave
         if (kind) {
             f32x16 s[NS];
             float mt = -INFINITY;
@@ -423,7 +441,26 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
                 }
         }
     }
-    const float l = half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
+    float l = half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
+    if constexpr (KS == 2) {
+        float* x = reinterpret_cast<float*>(smem) + rg * (16 * ND + 2) * 64;
+        __syncthreads();
+        if (part) {
+            half_put(x, o, lane);
+            x[16 * ND * 64 + lane] = m;
+            x[16 * ND * 64 + 64 + lane] = l;
+        }
+        __syncthreads();
+        if (!part) {
+            const float m1 = x[16 * ND * 64 + lane], l1 = x[16 * ND * 64 + 64 + lane], mn = fmaxf(m, m1);
+            const float f0 = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn), f1 = m1 == mn ? 1.f : __builtin_amdgcn_exp2f(m1 - mn);
+            half_add(x, o, f0, f1, lane);
+            l = l * f0 + l1 * f1;
+            m = mn;
+        }
+        __syncthreads();
+        if (part) return;
+    }
     const bool none = i >= len || (m == -INFINITY && l == 0.f);      // nothing visible (a NaN sum stays a NaN)
     // A non-finite V of a key that only some queries of a tile see has reached the others as 0 * V.  Where the result is not
     // finite, it is made again key by key, for the keys that each query sees.
@@ -470,18 +507,18 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
         }
     }
     if (p.lse && lane < 32 && i < p.N) p.lse[((long)b * p.Hq + h) * p.N + i] = none ? INFINITY : m + __log2f(l);
-    __syncthreads();
+    if constexpr (KS == 1) __syncthreads();
     const long at = ((long)b * p.N * p.Hq + h) * p.dh, ldg = (long)p.Hq * p.dh;
-    T* mine = lds + wave * 32 * C::LD;
+    T* mine = lds + rg * 32 * C::LD;
     put_rows<T, DP>(o, 1.f / l, none, mine, static_cast<T*>(p.out) + at, ldg, iw, p.N, p.dh, lane);
     if (sizeof(T) == 2 && p.o_lo) put_rows<T, DP, true>(o, 1.f / l, none, mine, static_cast<T*>(p.o_lo) + at, ldg, iw, p.N, p.dh, lane);
 }
 
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
-template <typename T, int DP, int NW, int BK, int WPE, bool FINE>
+template <typename T, int DP, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, NS = BK / 32, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
+    constexpr int NT = 64 * NW, RG = NW / KS, NS = BK / 32 / KS, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);
     const int id = xcd_order((int)blockIdx.x, p.total, p.run);
@@ -490,7 +527,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     const int r1 = uniform(id / p.G), g = id - r1 * p.G;
     const int bh = uniform(r1 / p.tiles), tq = r1 - bh * p.tiles;
     const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk, h = hk * p.G + g;
-    const int i0 = 32 * NW * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * wave;
+    const int part = KS == 1 ? 0 : uniform(wave / RG), rg = wave - part * RG;
+    const int i0 = 32 * RG * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * rg;
     const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
     const int i = iw + (lane & 31);
 
@@ -517,9 +555,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
         delta = half_sum(delta);
         const long at = ((long)b * p.Hq + h) * p.N + i;
         if (i < len) lse = p.lse[at];
-        if (lane < 32 && i < p.N) p.delta[at] = delta;
+        if (!part && lane < 32 && i < p.N) p.delta[at] = delta;
     }
-    const KeyTiles kt = key_tiles(p, i0, i0 + 32 * NW, len, BK);
+    const KeyTiles kt = key_tiles(p, i0, i0 + 32 * RG, len, BK);
     const RowRange rr = row_range(p, i, len);
     f32x16 dq[ND];
 #pragma unroll
@@ -537,7 +575,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
         sv.load(V, p.v.sn, j0, len, p.dh, lds + TILE, wave);
     }
     for (int it = 0; it < kt.n; ++it) {
-        const T* Ks = lds + (it & 1) * 2 * TILE;
+        const T* Ks = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
         const T* Vs = Ks + TILE;
         tile_ready();
         if (it + 1 < kt.n) {
@@ -546,8 +584,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
             sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
             sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
         }
-        const int j0 = BK * key_tile(kt, it);
-        const int kind = tile_kind(p, iw, 32, j0, BK, len);
+        const int j0 = BK * key_tile(kt, it) + 32 * NS * part;
+        const int kind = tile_kind(p, iw, 32, j0, 32 * NS, len);
         if (kind) {
 #pragma unroll
             for (int u = 0; u < NS; ++u) {
@@ -589,7 +627,15 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
         }
     }
     __syncthreads();
-    put_rows<T, DP>(dq, p.scale, i >= len, lds + wave * 32 * C::LD, static_cast<T*>(p.out) + ((long)b * p.N * p.Hq + h) * p.dh,
+    if constexpr (KS == 2) {
+        float* x = reinterpret_cast<float*>(smem) + rg * 16 * ND * 64;
+        if (part) half_put(x, dq, lane);
+        __syncthreads();
+        if (!part) half_add(x, dq, 1.f, 1.f, lane);
+        __syncthreads();
+        if (part) return;
+    }
+    put_rows<T, DP>(dq, p.scale, i >= len, lds + rg * 32 * C::LD, static_cast<T*>(p.out) + ((long)b * p.N * p.Hq + h) * p.dh,
                     (long)p.Hq * p.dh, iw, p.N, p.dh, lane);
 }
 
@@ -597,10 +643,10 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
 // every head of the group.  SINK: one wave, the 32 keys of a sinks' tile and a share of ALL the query tiles, fp32 partial
 // sums out (window_sink_sum_kernel adds the shares in order).
-template <typename T, int DP, int NW, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
+template <typename T, int DP, int NW, int KS, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, NS = BQ / 32, KD = DP / 16, ND = DP / 32, TILE = BQ * DP;
+    constexpr int NT = 64 * NW, RG = NW / KS, NS = BQ / 32 / KS, KD = DP / 16, ND = DP / 32, TILE = BQ * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (Q tile, dO tile), then of BQ (lse, D) each
     float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
@@ -626,7 +672,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk;
-    const int j0 = p.key0 + 32 * NW * tk, jw = j0 + 32 * wave, j = jw + (lane & 31);
+    const int part = KS == 1 ? 0 : uniform(wave / RG), rg = wave - part * RG;
+    const int j0 = p.key0 + 32 * RG * tk, jw = j0 + 32 * rg, j = jw + (lane & 31);
     const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
 
     Frag<T> kf[KD], vf[VLDS ? 1 : KD];
@@ -649,7 +696,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         int a = p.causal ? j0 : 0, e = len;
         if (p.w >= 0 && j0 >= p.S) {                     // (the sinks' tiles are seen from everywhere)
             a = max(a, j0 - p.w);
-            e = (int)min((long)e, (long)j0 + 32 * NW + p.w);
+            e = (int)min((long)e, (long)j0 + 32 * RG + p.w);
         }
         ta = a / BQ;
         nt = (e + BQ - 1) / BQ - ta;
@@ -665,7 +712,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
 
     loads_done();
     if constexpr (VLDS) {
-        Stager<T, DP, 32 * NW, NT> sv;
+        Stager<T, DP, 32 * RG, NT> sv;
         sv.init(p.v.sn, p.dh);
         sv.load(V, p.v.sn, j0, len, p.dh, Vs, wave);
     }
@@ -695,7 +742,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
             s = mma32(a, kf[kk], s);
             row_frag32<DP>(a, Ds, 32 * u, kk, lane);
             if constexpr (VLDS) {
-                row_frag32<DP>(v, Vs, 32 * wave, kk, lane);
+                row_frag32<DP>(v, Vs, 32 * rg, kk, lane);
                 dp = mma32(a, v, dp);
             } else {
                 dp = mma32(a, vf[kk], dp);
@@ -744,12 +791,12 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
     };
     if (it0 < it1) fetch(it0);
     for (int it = it0; it < it1; ++it) {
-        const T* Qs = lds + (it & 1) * 2 * TILE;
+        const T* Qs = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
         const T* Ds = Qs + TILE;
-        const float* ls = stat + (it & 1) * 2 * BQ;
+        const float* ls = stat + (it & 1) * 2 * BQ + 32 * NS * part;
         tile_ready();
         if (it + 1 < it1) fetch(it + 1);
-        const int i0 = BQ * (ta + it - uniform(it / nt) * nt);
+        const int i0 = BQ * (ta + it - uniform(it / nt) * nt) + 32 * NS * part;
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
             const int kind = jw < len ? tile_kind(p, i0 + 32 * u, 32, jw, 32, len) : 0;
@@ -769,7 +816,21 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         return;
     }
     __syncthreads();
-    T* mine = lds + wave * 32 * C::LD;
+    if constexpr (KS == 2) {
+        float* x = reinterpret_cast<float*>(smem) + rg * 32 * ND * 64;
+        if (part) {
+            half_put(x, dk, lane);
+            half_put(x + 16 * ND * 64, dv, lane);
+        }
+        __syncthreads();
+        if (!part) {
+            half_add(x, dk, 1.f, 1.f, lane);
+            half_add(x + 16 * ND * 64, dv, 1.f, 1.f, lane);
+        }
+        __syncthreads();
+        if (part) return;
+    }
+    T* mine = lds + rg * 32 * C::LD;
     const long at = ((long)b * p.N * p.Hk + hk) * p.dh, ldg = (long)p.Hk * p.dh;
     put_rows<T, DP>(dk, p.scale, j >= len, mine, static_cast<T*>(p.dk) + at, ldg, jw, p.N, p.dh, lane);
     put_rows<T, DP>(dv, 1.f, j >= len, mine, static_cast<T*>(p.dv) + at, ldg, jw, p.N, p.dh, lane);
@@ -811,19 +872,24 @@ namespace {
 
 struct Plan {                  // tiles of one call
     int dp;                    // staged head width: 32, 64, 96 or 128
-    int nwq, nwk;              // waves of a query / key workgroup
+    bool halves_q, halves_k;   // workgroups of 64 queries / keys whose rows are shared by two waves each, else of 128
     int sink_keys;             // keys that the sinks' launch takes (a multiple of 32, 0: none)
     int chunks, per_chunk;
     bool fine;                 // bf16: P and dS as two bf16 each
 };
 constexpr long FINE = 1 << 17;
-constexpr int SINK_BQ = 32;
+constexpr int SINK_BQ = 32, SINK_ITEMS = 24;
 constexpr int NARROW = 256;
 
-// Fewer, larger workgroups read K and V fewer times; they are halved where the large ones would leave CUs without work.
-int waves_for(long rows_tiles_of_128) { return rows_tiles_of_128 >= 512 ? 4 : 2; }
+// Up to how many workgroups of 128 rows there are, that workgroups of 64 with two waves a row, each with half of the other axis,
+// are faster.  One of 128 takes as long as its longest row, whatever the other CUs do: few of them leave CUs, and a second
+// round of them most of its CUs, waiting.  Halves read every tile for half the rows.  fp32, 16 heads x 1001 tokens of 80, forward
+// and backward: one sequence 68 + 205 us against 120 + 390, three 200 + 608 against 209 + 749, four 265 + 808 against 211 +
+// 759; causal, four of 1024: 201 + 605 against 210 + 746.  bf16, 16 x 1024: heads of 128 24 + 59 against 31 + 93, two sequences
+// 31 + 99 against 34 + 95, three 47 + 149 against 41 + 118; of 64 three 26 + 75 against 28 + 76, four 33 + 92 against 30 + 83.
+long halves_up_to(int dtype, int dp, bool uneven) { return dtype == VITK_F32 ? (uneven ? 512 : 384) : (dp <= 64 ? 384 : 256); }
 
-Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S) {
+Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bool uneven) {
     Plan pl;
     pl.dp = (dh + 31) / 32 * 32;
     // P and dS are rounded to bf16 for their products, an error of the size of the results' own rounding as long as many share in
@@ -833,12 +899,17 @@ Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S) {
     // 21.5).
     const long keys = w < 0 ? N : (2L * w + 1 + S < N ? 2L * w + 1 + S : N);
     pl.fine = dtype == VITK_BF16 && (long)B * Hq * N * keys <= FINE;
-    pl.nwq = waves_for((long)B * Hq * ((N + 127) / 128));
-    pl.nwk = waves_for((long)B * Hk * ((N + 127) / 128));
-    // The sinks' keys are seen by all N queries, other keys by 2 w + 1: where that is over four times more, they get a launch of
-    // their own, whose workgroups share the queries; else they stay in the ordinary one (16 x 577 tokens, window 64: 45 us in
-    // all against 33 + 14 + 7).
-    pl.sink_keys = w >= 0 && S > 0 && N > 4L * (128 + 2L * w) ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
+    const long tq = (long)B * Hq * ((N + 127) / 128), tk = (long)B * Hk * ((N + 127) / 128), most = halves_up_to(dtype, pl.dp, uneven);
+    pl.halves_q = pl.fine || tq <= most;
+    pl.halves_k = pl.fine || tk <= most;
+    // The sinks' keys are seen by all N queries, the 128 of another tile by `near` of them.  Where that is over four times more, or
+    // so much that the ordinary launch would wait for the sinks' tiles, they get a launch of their own, whose workgroups share
+    // the queries, and a sum; else they go first in the ordinary one (16 x 577 tokens x 12 heads, window 64: 39 us in all
+    // against 33 + 14 + 7; backward of 1 x 577 x 12: 26 against 31, of 1001 tokens x 8 heads in groups of 4, causal window of
+    // 100: 85 against 44, fp32 314 against 125).
+    const long near = 128 + 2L * w;
+    const bool apart = N > 4 * near || ((N - near) * 256 > near * tk && (N - near) * (Hq / Hk) > 32 * SINK_ITEMS);
+    pl.sink_keys = w >= 0 && S > 0 && apart ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
     if ((long)B * Hk * pl.sink_keys >= (1L << 22)) pl.sink_keys = 0;     // (their sum would be more than 2^32 threads)
     pl.chunks = pl.per_chunk = 0;
     if (pl.sink_keys) {
@@ -893,70 +964,78 @@ unsigned xcd_grid(WindowParams& p, int total) {
     return (unsigned)((total + round - 1) / round * round);
 }
 
-template <typename T, int DP, int NW, int BK, bool FINE = false> void run_fwd_tiles(WindowParams p, hipStream_t st) {
-    constexpr int WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;           // one wave a SIMD where two would spill
-    p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
+constexpr int NW = 4;
+// bytes of LDS that `waves` groups of 32 rows need to leave through (put_rows), after which `n` accumulators of theirs were joined
+template <typename T, int DP> size_t rows_lds(int groups, int n) {
+    const size_t rows = 32 * groups * WCfg<T, DP>::LD * sizeof(T), join = n ? (size_t)groups * (DP / 2 * n + 2) * 64 * sizeof(float) : 0;
+    return rows > join ? rows : join;
+}
+template <typename T, int DP, int KS, int BK, bool FINE = false> void run_fwd_tiles(WindowParams p, hipStream_t st) {
+    constexpr int WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;             // one wave a SIMD where two would spill
+    p.tiles = (p.N + 32 * RG - 1) / (32 * RG);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
-    const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
-    const size_t lds = tiles > rows ? tiles : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, BK, WPE, FINE>), lds);
-    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    const size_t lds = std::max<size_t>(4 * BK * DP * sizeof(T), rows_lds<T, DP>(RG, KS - 1));
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, KS, BK, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
 // Key tiles of 64 in bf16; of 32 where the window is narrow and a tile of 64 would be mostly edge (16 x 577 tokens x 12 heads of
 // 64, window 64 on both sides: 24.1 us against 27.1, window 256: 33.5 against 34.7; 2 x 8192 x 16 heads of 128, causal window
 // of 512: 124.4 against 123.0, 16384 x 16, of 1024: 222 against 190).
 template <typename T, int DP> void run_fwd(const WindowParams& p, const Plan& pl, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        const bool narrow = p.w >= 0 && p.w <= NARROW;
-        if (pl.fine) return narrow ? run_fwd_tiles<T, DP, 2, 32, true>(p, st) : run_fwd_tiles<T, DP, 2, 64, true>(p, st);
-        if (!narrow) return pl.nwq == 4 ? run_fwd_tiles<T, DP, 4, 64>(p, st) : run_fwd_tiles<T, DP, 2, 64>(p, st);
+        if (pl.fine) return run_fwd_tiles<T, DP, 2, 64, true>(p, st);
     }
-    if (pl.nwq == 4) run_fwd_tiles<T, DP, 4, 32>(p, st);
-    else run_fwd_tiles<T, DP, 2, 32>(p, st);
+    if (pl.halves_q) return run_fwd_tiles<T, DP, 2, 64>(p, st);
+    if constexpr (sizeof(T) == 2) {
+        if (p.w < 0 || p.w > NARROW) return run_fwd_tiles<T, DP, 1, 64>(p, st);
+    }
+    run_fwd_tiles<T, DP, 1, 32>(p, st);
 }
-template <typename T, int DP, int NW, bool FINE = false> void run_dq(WindowParams p, hipStream_t st) {
-    constexpr int BK = 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2;
-    p.tiles = (p.N + 32 * NW - 1) / (32 * NW);
+template <typename T, int DP, int KS, bool FINE> void run_dq(WindowParams p, hipStream_t st) {
+    constexpr int BK = 32 * KS, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;
+    p.tiles = (p.N + 32 * RG - 1) / (32 * RG);
     const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
-    const size_t tiles = 4 * BK * DP * sizeof(T), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
-    const size_t lds = tiles > rows ? tiles : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, BK, WPE, FINE>), lds);
-    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    const size_t lds = std::max<size_t>(4 * BK * DP * sizeof(T), rows_lds<T, DP>(RG, KS - 1));
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, KS, BK, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
-template <typename T, int DP, int NW, int BQ, bool SINK, bool FINE = false> void run_dkv(WindowParams p, int tiles, hipStream_t st) {
+template <typename T, int DP, int W, int KS, int BQ, bool SINK, bool FINE> void run_dkv(WindowParams p, int keys, hipStream_t st) {
     // V rows in LDS where they, K's and both accumulators do not fit the registers of two waves a SIMD
     constexpr bool VLDS = sizeof(T) == 2 && DP >= 96 && !SINK;
-    constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK || (FINE && DP == 128) ? 1 : 2;
-    p.tiles = tiles;
-    p.heavy = SINK ? 0 : (p.S > p.key0 ? (p.S - p.key0 + 32 * NW - 1) / (32 * NW) : 0);
-    if (p.heavy >= tiles) p.heavy = 0;                   // nothing but sinks: all alike
-    const unsigned grid = xcd_grid(p, p.B * p.Hk * (tiles - p.heavy) * (SINK ? p.chunks : 1)) + (p.heavy * p.B * p.Hk + 7) / 8 * 8;
-    const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * NW * DP * sizeof(T) : 0), rows = 32 * NW * WCfg<T, DP>::LD * sizeof(T);
-    const size_t lds = tl > rows ? tl : rows;
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE, FINE>), lds);
-    hipLaunchKernelGGL((window_dkv_kernel<T, DP, NW, BQ, SINK, VLDS, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK || (FINE && DP == 128) ? 1 : 2, RG = W / KS;
+    p.tiles = (keys + 32 * RG - 1) / (32 * RG);
+    p.heavy = SINK ? 0 : (p.S > p.key0 ? (p.S - p.key0 + 32 * RG - 1) / (32 * RG) : 0);
+    if (p.heavy >= p.tiles) p.heavy = 0;                 // nothing but sinks: all alike
+    const unsigned grid = xcd_grid(p, p.B * p.Hk * (p.tiles - p.heavy) * (SINK ? p.chunks : 1)) + (p.heavy * p.B * p.Hk + 7) / 8 * 8;
+    const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * RG * DP * sizeof(T) : 0);
+    const size_t lds = std::max<size_t>(tl, rows_lds<T, DP>(RG, 2 * (KS - 1)));
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, W, KS, BQ, SINK, VLDS, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_dkv_kernel<T, DP, W, KS, BQ, SINK, VLDS, WPE, FINE>), dim3(grid), dim3(64 * W), lds, st, p);
 }
 template <typename T, int DP, bool FINE> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
     constexpr int BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     p.out = dq;
-    if (!FINE && pl.nwq == 4) run_dq<T, DP, 4>(p, st);
-    else run_dq<T, DP, 2, FINE>(p, st);
+    if constexpr (!FINE) {
+        if (!pl.halves_q) run_dq<T, DP, 1, FINE>(p, st);
+    }
+    if (pl.halves_q) run_dq<T, DP, 2, FINE>(p, st);
     if (pl.sink_keys) {
         WindowParams s = p;
         s.key0 = 0;
         s.chunks = pl.chunks;
         s.per_chunk = pl.per_chunk;
-        run_dkv<T, DP, 1, SINK_BQ, true, FINE>(s, pl.sink_keys / 32, st);
+        run_dkv<T, DP, 1, 1, SINK_BQ, true, FINE>(s, pl.sink_keys, st);
         s.tiles = pl.sink_keys / 32;
         hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles * 2 * (DP / 2))), dim3(256),
                            0, st, s);
     }
     p.key0 = pl.sink_keys;
     const int rest = p.N - pl.sink_keys;
-    if (rest > 0) {
-        if (!FINE && pl.nwk == 4) run_dkv<T, DP, 4, BQ, false>(p, (rest + 127) / 128, st);
-        else run_dkv<T, DP, 2, BQ, false, FINE>(p, (rest + 63) / 64, st);
+    if (rest <= 0) return;
+    if constexpr (!FINE) {
+        if (!pl.halves_k) run_dkv<T, DP, NW, 1, BQ, false, FINE>(p, rest, st);
     }
+    if (pl.halves_k) run_dkv<T, DP, NW, 2, 64, false, FINE>(p, rest, st);
 }
 template <typename T, int DP> void run_bwd(const WindowParams& p, const Plan& pl, void* dq, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
@@ -988,7 +1067,7 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     p.out = out;
     p.o_lo = out_lo;
     p.lse = lse;
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal || p.w >= 0 || lengths);
 #define GO(T, D) run_fwd<T, D>(p, pl, stream)
 #define BY_DP(T) switch (pl.dp) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 96: GO(T, 96); break; default: GO(T, 128); break; }
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
@@ -1002,7 +1081,7 @@ extern "C" long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, in
     if (B <= 0 || N <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || dh < 8 || dh > 128 || sinks < 0) return 0;
     WindowParams p = {};
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, 0, 1.f, nullptr);
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, true);
     return ((long)B * Hq * N + 3) / 4 * 16 + part_floats(pl, B, Hk) * 4;
 }
 
@@ -1036,7 +1115,7 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     p.part = p.delta + ((long)B * Hq * N + 3) / 4 * 4;
     p.dk = dk;
     p.dv = dv;
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal || p.w >= 0 || lengths);
 #define GO(T, D) run_bwd<T, D>(p, pl, dq, stream)
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
     else { BY_DP(float) }
