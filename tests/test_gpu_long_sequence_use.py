@@ -160,3 +160,39 @@ def test_small_calls_round_once(monkeypatch, case):
     want = R.window_attention(*(t.detach() for t in ins), window, sinks, causal, dh ** -0.5, None, do)
     for t, x in got.items():
         R.within(x, want[t][0], want[t][1] + 2.0 ** -8 * want[t][0].abs(), t)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+def test_far_rows(dtype):
+    """Tokens just under and over 16 MiB apart (the larger stride is copied, not refused)."""
+    from vit_amd import functional as VF
+    near = torch.randn(1, 5, 2, 32, generator=_gen(47), device='cuda').to(dtype)
+    want = VF.window_attention(near, near, near, 2, causal=True)
+    for stride in ((1 << 24) // near.element_size() - 64, (1 << 24) // near.element_size() + 64):
+        store = torch.full((4 * stride + 64,), float('nan'), dtype=dtype, device='cuda')
+        far = torch.as_strided(store, near.shape, (0, stride, 32, 1))
+        far.copy_(near)
+        assert torch.equal(VF.window_attention(far, far, far, 2, causal=True), want)
+        kc = torch.zeros(1, 2, 5, 32, dtype=dtype, device='cuda')
+        vc = torch.zeros_like(kc)
+        VF.window_cache_fill(far, far, kc, vc)
+        assert torch.equal(kc, near.transpose(1, 2)) and torch.equal(vc, kc)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('case', [(1, 1201, 4, 1, 128, 40, 5), (2, 1001, 6, 2, 80, 100, 33), (1, 2100, 2, 2, 64, 10, 70),
+                                  (3, 700, 4, 4, 24, 3, 1)], ids=str)
+def test_sinks_of_their_own_launch(case, dtype):
+    """Few rows and sinks that every query sees: two waves a row, and the sinks' keys in workgroups that share the queries."""
+    from vit_amd import functional as VF
+    B, N, Hq, Hk, dh, window, sinks = case
+    g = _gen(48)
+    q, k, v, do = (torch.randn(B, N, h, dh, generator=g, device='cuda').to(dtype) for h in (Hq, Hk, Hk, Hq))
+    lengths = torch.randint(1, N + 1, (B,), generator=g, device='cuda', dtype=torch.int32)
+    for causal, n in ((True, None), (False, lengths)):
+        ins = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o = VF.window_attention(*ins, window, sinks=sinks, causal=causal, lengths=n)
+        got = dict(zip(('o', 'dq', 'dk', 'dv'), (o.detach(), *torch.autograd.grad(o, ins, do))))
+        want = R.window_attention(q, k, v, window, sinks, causal, dh ** -0.5, n, do)
+        for t, x in got.items():
+            R.within(x, *want[t], t)

@@ -173,8 +173,12 @@ __device__ __forceinline__ void tile_ready() {
 }
 // ROWS floats of the rows' statistics, the same way (by one wave)
 template <int ROWS> __device__ __forceinline__ void load_stat(const float* g, int row0, int hi, float* lds, int lane) {
-    const int n = min(hi - row0, ROWS);
-    if (ROWS == 64 || lane < ROWS) load_to_lds<4>(g + row0, n > 0 ? 4u * n : 0u, 4u * lane, lds);
+    static_assert(ROWS == 32 || ROWS % 64 == 0, "whole waves of rows, or half of one");
+#pragma unroll
+    for (int r = 0; r < ROWS; r += 64) {
+        const int n = min(hi - row0 - r, ROWS - r);
+        if (ROWS != 32 || lane < 32) load_to_lds<4>(g + row0 + r, n > 0 ? 4u * n : 0u, 4u * lane, lds + r);
+    }
 }
 
 // the other half-wave's value joined in: every lane gets f of lanes l and l ^ 32
@@ -641,8 +645,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 
 // --------------------------------------------------------------------------------------------- backward: dk and dv
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
-// every head of the group.  SINK: one wave, the 32 keys of a sinks' tile and a share of ALL the query tiles, fp32 partial
-// sums out (window_sink_sum_kernel adds the shares in order).
+// every head of the group.  KS waves share 32 keys, each with its own part of every query tile.  SINK: the 32 keys of a sinks'
+// tile and a share of ALL the query tiles, each wave's sums out in fp32 (window_sink_sum_kernel adds the shares in order).
 template <typename T, int DP, int NW, int KS, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
     using C = WCfg<T, DP>;
@@ -804,7 +808,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         }
     }
     if (SINK) {
-        float* o = p.part + (long)id * 2 * DP * 32;
+        float* o = p.part + ((long)id * KS + part) * 2 * DP * 32;
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -874,11 +878,13 @@ struct Plan {                  // tiles of one call
     int dp;                    // staged head width: 32, 64, 96 or 128
     bool halves_q, halves_k;   // workgroups of 64 queries / keys whose rows are shared by two waves each, else of 128
     int sink_keys;             // keys that the sinks' launch takes (a multiple of 32, 0: none)
-    int chunks, per_chunk;
+    int chunks, per_chunk;     // workgroups a sinks' tile, query tiles each of them takes
+    int shares;                // partial sums that they leave
     bool fine;                 // bf16: P and dS as two bf16 each
 };
 constexpr long FINE = 1 << 17;
-constexpr int SINK_BQ = 32, SINK_ITEMS = 24;
+constexpr int SINK_ITEMS = 24;
+constexpr int sink_waves(int bytes_of_a_row) { return bytes_of_a_row <= 128 ? 4 : 2; }       // 4 tiles of 32 rows each for them in LDS
 constexpr int NARROW = 256;
 
 // Up to how many workgroups of 128 rows there are, that workgroups of 64 with two waves a row, each with half of the other axis,
@@ -911,19 +917,21 @@ Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bo
     const bool apart = N > 4 * near || ((N - near) * 256 > near * tk && (N - near) * (Hq / Hk) > 32 * SINK_ITEMS);
     pl.sink_keys = w >= 0 && S > 0 && apart ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
     if ((long)B * Hk * pl.sink_keys >= (1L << 22)) pl.sink_keys = 0;     // (their sum would be more than 2^32 threads)
-    pl.chunks = pl.per_chunk = 0;
+    pl.chunks = pl.per_chunk = pl.shares = 0;
     if (pl.sink_keys) {
-        // about 1024 one-wave workgroups, at least 4 query tiles each
-        const long items = (long)((N + SINK_BQ - 1) / SINK_BQ) * (Hq / Hk), sets = (long)B * Hk * (pl.sink_keys / 32);
-        long want = (1024 + sets - 1) / sets;
-        long per = (items + want - 1) / want;
-        if (per < 4) per = 4;
+        // workgroups of waves that share the 32 keys and have their own queries each, about 1024 waves in all and 2 tiles or more a
+        // workgroup: all of q and do is read once (16384 tokens x 16 heads of 128, 134 MB: 36 us; one-wave workgroups 34; 3 x
+        // 1001 x 8 heads in groups of 4, fp32: the backward 264 us against 293)
+        const int waves = sink_waves(pl.dp * (dtype == VITK_F32 ? 4 : 2)), rows = 32 * waves;
+        const long items = (long)((N + rows - 1) / rows) * (Hq / Hk), sets = (long)B * Hk * (pl.sink_keys / 32);
+        const long want = (1024 / waves + sets - 1) / sets, per = std::max((items + want - 1) / want, 2L);
         pl.per_chunk = (int)per;
         pl.chunks = (int)((items + per - 1) / per);
+        pl.shares = pl.chunks * waves;
     }
     return pl;
 }
-long part_floats(const Plan& pl, int B, int Hk) { return (long)B * Hk * (pl.sink_keys / 32) * pl.chunks * 2 * pl.dp * 32; }
+long part_floats(const Plan& pl, int B, int Hk) { return (long)B * Hk * (pl.sink_keys / 32) * pl.shares * 2 * pl.dp * 32; }
 
 int check_window(const char* what, int dtype, int B, int N, int Hq, int Hk, int dh, float scale, int sinks) {
     VITK_CHECK_ARG(dtype == VITK_F32 || dtype == VITK_BF16, "%s: bad dtype %d", what, dtype);
@@ -940,7 +948,7 @@ int check_view(const char* what, const char* name, const View& v, int dtype) {
     const int per = dtype == VITK_F32 ? 4 : 8;
     VITK_CHECK_ARG(v.p && (reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.sb % per == 0 && v.sn % per == 0 && v.sh % per == 0,
                    "%s: %s must be 16-byte aligned, its strides too", what, name);
-    VITK_CHECK_ARG(v.sn >= 0 && v.sn < (1L << 23), "%s: the tokens of %s are too far apart", what, name);    // 64 rows under 2 GiB
+    VITK_CHECK_ARG(v.sn >= 0 && v.sn < (1L << 20) * per, "%s: the tokens of %s are too far apart", what, name);    // 128 rows under 2 GiB
     return VITK_OK;
 }
 void fill_params(WindowParams& p, int B, int N, int Hq, int Hk, int dh, int w, int S, int causal, float scale, const int* lengths) {
@@ -1024,8 +1032,10 @@ template <typename T, int DP, bool FINE> void run_bwd(WindowParams p, const Plan
         s.key0 = 0;
         s.chunks = pl.chunks;
         s.per_chunk = pl.per_chunk;
-        run_dkv<T, DP, 1, 1, SINK_BQ, true, FINE>(s, pl.sink_keys, st);
+        constexpr int W = sink_waves(DP * sizeof(T));
+        run_dkv<T, DP, W, W, 32 * W, true, FINE>(s, pl.sink_keys, st);
         s.tiles = pl.sink_keys / 32;
+        s.chunks = pl.shares;
         hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles * 2 * (DP / 2))), dim3(256),
                            0, st, s);
     }

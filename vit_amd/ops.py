@@ -538,10 +538,11 @@ def _heads(t, what):
 
 
 def _aligned_heads(t):
-    """16-byte aligned rows, as the attention kernels read them: ``t`` itself, or a copy."""
-    per = 16 // t.element_size()
-    s = t.stride()
-    if s[-1] == 1 and t.data_ptr() % 16 == 0 and not any(x % per for x in s[:-1]):
+    """16-byte aligned rows, neighbours of a sequence under 16 MiB apart, as the attention kernels read them: ``t`` itself, or a
+    copy."""
+    es, s = t.element_size(), t.stride()
+    per = 16 // es
+    if s[-1] == 1 and t.data_ptr() % 16 == 0 and not any(x % per for x in s[:-1]) and (len(s) < 4 or s[1] * es < 1 << 24):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
