@@ -112,6 +112,9 @@ struct WindowParams {
     int key0;                     // keys' kernel: first key (the sinks before it have their own launch)
     int heavy;                    // keys' kernel: how many of a sequence's tiles, the first ones, hold sinks
     int chunks, per_chunk;        // sinks' launch: query tiles are dealt to `chunks` workgroups
+    // order of the pieces of work: tiles within a (sequence, key head), or (by_tile) all sequences' and heads' tiles of one place,
+    // the long ones first; the group's heads innermost
+    int by_tile, inner;           // inner: how many of the inner kind there are
     int run;                      // consecutive pieces of work an XCD takes at a time
     int total;                    // workgroups that have work (the grid is rounded up to whole rounds of the 8 XCDs)
     float scale, sc2;             // sc2 = scale * log2(e)
@@ -328,12 +331,12 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     const int id = xcd_order((int)blockIdx.x, p.total, p.run);
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // order of the work: the group's heads, then query tiles, then (sequence, key head); causal: long rows first
     const int r1 = uniform(id / p.G), g = id - r1 * p.G;
-    const int bh = uniform(r1 / p.tiles), tq = r1 - bh * p.tiles;
+    const int major = uniform(r1 / p.inner), minor = r1 - major * p.inner;
+    const int bh = p.by_tile ? minor : major, tq = p.by_tile ? major : minor;
     const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk, h = hk * p.G + g;
     const int part = KS == 1 ? 0 : uniform(wave / RG), rg = wave - part * RG;
-    const int i0 = 32 * RG * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * rg;
+    const int i0 = 32 * RG * (p.by_tile ? p.tiles - 1 - tq : tq), iw = i0 + 32 * rg;
     const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
     const int i = iw + (lane & 31);
 
@@ -529,10 +532,11 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r1 = uniform(id / p.G), g = id - r1 * p.G;
-    const int bh = uniform(r1 / p.tiles), tq = r1 - bh * p.tiles;
+    const int major = uniform(r1 / p.inner), minor = r1 - major * p.inner;
+    const int bh = p.by_tile ? minor : major, tq = p.by_tile ? major : minor;
     const int b = uniform(bh / p.Hk), hk = bh - b * p.Hk, h = hk * p.G + g;
     const int part = KS == 1 ? 0 : uniform(wave / RG), rg = wave - part * RG;
-    const int i0 = 32 * RG * (p.causal ? p.tiles - 1 - tq : tq), iw = i0 + 32 * rg;
+    const int i0 = 32 * RG * (p.by_tile ? p.tiles - 1 - tq : tq), iw = i0 + 32 * rg;
     const int len = p.lengths ? uniform(max(0, min(p.lengths[b], p.N))) : p.N;
     const int i = iw + (lane & 31);
 
@@ -669,9 +673,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
             r1 = uniform(r1 / p.chunks);
             chunk -= r1 * p.chunks;
         }
-        const int rest = p.tiles - p.heavy;
-        bh = uniform(r1 / rest);
-        tk = p.heavy + r1 - bh * rest;
+        const int major = uniform(r1 / p.inner), minor = r1 - major * p.inner;
+        bh = p.by_tile ? minor : major;
+        tk = p.by_tile ? (p.causal ? p.heavy + major : p.tiles - 1 - major) : p.heavy + minor;
     }
     if (id < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -895,7 +899,7 @@ constexpr int NARROW = 256;
 // 31 + 99 against 34 + 95, three 47 + 149 against 41 + 118; of 64 three 26 + 75 against 28 + 76, four 33 + 92 against 30 + 83.
 long halves_up_to(int dtype, int dp, bool uneven) { return dtype == VITK_F32 ? (uneven ? 512 : 384) : (dp <= 64 ? 384 : 256); }
 
-Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bool uneven) {
+Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bool causal, bool uneven) {
     Plan pl;
     pl.dp = (dh + 31) / 32 * 32;
     // P and dS are rounded to bf16 for their products, an error of the size of the results' own rounding as long as many share in
@@ -913,7 +917,7 @@ Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bo
     // the queries, and a sum; else they go first in the ordinary one (16 x 577 tokens x 12 heads, window 64: 39 us in all
     // against 33 + 14 + 7; backward of 1 x 577 x 12: 26 against 31, of 1001 tokens x 8 heads in groups of 4, causal window of
     // 100: 85 against 44, fp32 314 against 125).
-    const long near = 128 + 2L * w;
+    const long near = 128 + (causal ? 1L : 2L) * w;
     const bool apart = N > 4 * near || ((N - near) * 256 > near * tk && (N - near) * (Hq / Hk) > 32 * SINK_ITEMS);
     pl.sink_keys = w >= 0 && S > 0 && apart ? ((S < N ? S : N) + 31) / 32 * 32 : 0;
     if ((long)B * Hk * pl.sink_keys >= (1L << 22)) pl.sink_keys = 0;     // (their sum would be more than 2^32 threads)
@@ -960,17 +964,22 @@ void fill_params(WindowParams& p, int B, int N, int Hq, int Hk, int dh, int w, i
     p.scale = scale;
     p.sc2 = scale * 1.4426950408889634f;
 }
-// Sets p.total and p.run; the grid that goes with them.  Pieces of equal work: an eighth of them in a row to each XCD (causal
-// 16384 x 128, groups of 4 heads: 180 us forward, with runs of 64 or 16 pieces 194).  Pieces that differ (sequences of
-// different lengths, causal rows without a window): runs of 16, fewer where there is little work (three sequences of 1001
-// tokens and less, fp32: forward 167 us, with an eighth in a row 219).
-unsigned xcd_grid(WindowParams& p, int total) {
+// Sets the order of the (tile, sequence, key head) pieces of `each` neighbours, and the grid that goes with it.  By tile, the long
+// ones first, dealt to the XCDs in turn: where pieces differ (sequences of different lengths, causal rows without a window:
+// 8192 tokens x 16 heads of 128, groups of 4, forward and backward 290 + 1214 us; in runs of 16 to each XCD, some of which then
+// had all the long ones, 405 + 2147), and where heads are a multiple of 8, so that a head stays on one XCD (16 x 577 x 12 heads
+// of 64, window 64: 20 + 62 us against 22 + 66).  Else an eighth of the pieces in a row to each XCD (16384 tokens, groups of 4
+// heads of 128, window 1024: 181 + 555 us against 183 + 567).
+unsigned xcd_grid(WindowParams& p, int tiles, int each, bool by_tile) {
+    const int heads = p.B * p.Hk, total = heads * tiles * each;
     p.total = total;
-    p.run = (total + 7) / 8;
-    if (p.lengths || (p.causal && p.w < 0)) p.run = total / 32 < 1 ? 1 : (total / 32 > 16 ? 16 : total / 32);
+    p.by_tile = by_tile;
+    p.inner = by_tile ? heads : tiles;
+    p.run = by_tile ? each : (total + 7) / 8;
     const long round = 8L * p.run;
     return (unsigned)((total + round - 1) / round * round);
 }
+bool by_tile(const WindowParams& p) { return p.lengths || (p.causal && p.w < 0) || (long)p.B * p.Hk % 8 == 0; }
 
 constexpr int NW = 4;
 // bytes of LDS that `waves` groups of 32 rows need to leave through (put_rows), after which `n` accumulators of theirs were joined
@@ -981,7 +990,7 @@ template <typename T, int DP> size_t rows_lds(int groups, int n) {
 template <typename T, int DP, int KS, int BK, bool FINE = false> void run_fwd_tiles(WindowParams p, hipStream_t st) {
     constexpr int WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;             // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * RG - 1) / (32 * RG);
-    const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
+    const unsigned grid = xcd_grid(p, p.tiles, p.G, by_tile(p));
     const size_t lds = std::max<size_t>(4 * BK * DP * sizeof(T), rows_lds<T, DP>(RG, KS - 1));
     vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, KS, BK, WPE, FINE>), lds);
     hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
@@ -1002,7 +1011,7 @@ template <typename T, int DP> void run_fwd(const WindowParams& p, const Plan& pl
 template <typename T, int DP, int KS, bool FINE> void run_dq(WindowParams p, hipStream_t st) {
     constexpr int BK = 32 * KS, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;
     p.tiles = (p.N + 32 * RG - 1) / (32 * RG);
-    const unsigned grid = xcd_grid(p, p.B * p.Hq * p.tiles);
+    const unsigned grid = xcd_grid(p, p.tiles, p.G, by_tile(p));
     const size_t lds = std::max<size_t>(4 * BK * DP * sizeof(T), rows_lds<T, DP>(RG, KS - 1));
     vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, KS, BK, WPE, FINE>), lds);
     hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
@@ -1014,7 +1023,7 @@ template <typename T, int DP, int W, int KS, int BQ, bool SINK, bool FINE> void 
     p.tiles = (keys + 32 * RG - 1) / (32 * RG);
     p.heavy = SINK ? 0 : (p.S > p.key0 ? (p.S - p.key0 + 32 * RG - 1) / (32 * RG) : 0);
     if (p.heavy >= p.tiles) p.heavy = 0;                 // nothing but sinks: all alike
-    const unsigned grid = xcd_grid(p, p.B * p.Hk * (p.tiles - p.heavy) * (SINK ? p.chunks : 1)) + (p.heavy * p.B * p.Hk + 7) / 8 * 8;
+    const unsigned grid = xcd_grid(p, p.tiles - p.heavy, SINK ? p.chunks : 1, !SINK && by_tile(p)) + (p.heavy * p.B * p.Hk + 7) / 8 * 8;
     const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * RG * DP * sizeof(T) : 0);
     const size_t lds = std::max<size_t>(tl, rows_lds<T, DP>(RG, 2 * (KS - 1)));
     vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, W, KS, BQ, SINK, VLDS, WPE, FINE>), lds);
@@ -1077,7 +1086,7 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     p.out = out;
     p.o_lo = out_lo;
     p.lse = lse;
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal || p.w >= 0 || lengths);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal, p.causal || p.w >= 0 || lengths);
 #define GO(T, D) run_fwd<T, D>(p, pl, stream)
 #define BY_DP(T) switch (pl.dp) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 96: GO(T, 96); break; default: GO(T, 128); break; }
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
@@ -1091,8 +1100,10 @@ extern "C" long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, in
     if (B <= 0 || N <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || dh < 8 || dh > 128 || sinks < 0) return 0;
     WindowParams p = {};
     fill_params(p, B, N, Hq, Hk, dh, window, sinks, 0, 1.f, nullptr);
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, true);
-    return ((long)B * Hq * N + 3) / 4 * 16 + part_floats(pl, B, Hk) * 4;
+    long part = 0;                                       // causal or not, whichever leaves more
+    for (int causal = 0; causal < 2; ++causal)
+        part = std::max(part, part_floats(make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, causal, true), B, Hk));
+    return ((long)B * Hq * N + 3) / 4 * 16 + part * 4;
 }
 
 extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
@@ -1125,7 +1136,7 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     p.part = p.delta + ((long)B * Hq * N + 3) / 4 * 4;
     p.dk = dk;
     p.dv = dv;
-    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal || p.w >= 0 || lengths);
+    const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal, p.causal || p.w >= 0 || lengths);
 #define GO(T, D) run_bwd<T, D>(p, pl, dq, stream)
     if (dtype == VITK_BF16) { BY_DP(__bf16) }
     else { BY_DP(float) }
