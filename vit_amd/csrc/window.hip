@@ -196,15 +196,15 @@ __device__ __forceinline__ float half_sum(float x) {
 
 // this wave's 32 rows of a strided matrix as fragments (rows outside [0, hi) are zero).  Loads without a branch, so that all are
 // on their way together: a lane with nothing to read reads the first element and drops it.
-template <typename T, int DP>
-__device__ __forceinline__ void own_rows(Frag<T> (&f)[DP / 16], const T* g, long sn, int row, int hi, int dh, int lane) {
+template <typename T, int KD>
+__device__ __forceinline__ void own_rows(Frag<T> (&f)[KD], const T* g, long sn, int row, int hi, int dh, int lane) {
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
+    for (int kk = 0; kk < KD; ++kk) {
         const int d = 16 * kk + 8 * (lane >> 5);
         frag_load(f[kk], g + (row < hi && d < dh ? (long)row * sn + d : 0));
     }
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk)
+    for (int kk = 0; kk < KD; ++kk)
         if (!(row < hi && 16 * kk + 8 * (lane >> 5) < dh)) frag_zero(f[kk]);
 }
 
@@ -322,10 +322,11 @@ template <int ND> __device__ __forceinline__ void half_add(const float* x, f32x1
 
 // ---------------------------------------------------------------------------------------------------------- forward
 // A wave owns 32 queries; KS = 2: two waves share them, each with one half of every tile of keys.
-template <typename T, int DP, int NW, int KS, int BK, int WPE, bool FINE>
+template <typename T, int HW, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowParams p) {
+    constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, RG = NW / KS, NS = BK / 32 / KS, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
+    constexpr int NT = 64 * NW, RG = NW / KS, NS = BK / 32 / KS, KD = HW / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (K tile, V tile)
     const int id = xcd_order((int)blockIdx.x, p.total, p.run);
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     const T* K = static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh;
     const T* V = static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh;
     Frag<T> qf[KD];
-    own_rows<T, DP>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
+    own_rows<T, KD>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
 
     const KeyTiles kt = key_tiles(p, i0, i0 + 32 * RG, len, BK);
     const RowRange rr = row_range(p, i, len);
@@ -522,10 +523,11 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
 }
 
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
-template <typename T, int DP, int NW, int KS, int BK, int WPE, bool FINE>
+template <typename T, int HW, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowParams p) {
+    constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, RG = NW / KS, NS = BK / 32 / KS, KD = DP / 16, ND = DP / 32, TILE = BK * DP;
+    constexpr int NT = 64 * NW, RG = NW / KS, NS = BK / 32 / KS, KD = HW / 16, ND = DP / 32, TILE = BK * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);
     const int id = xcd_order((int)blockIdx.x, p.total, p.run);
@@ -543,16 +545,16 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     const T* K = static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh;
     const T* V = static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh;
     Frag<T> qf[KD], df[KD];
-    own_rows<T, DP>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
-    own_rows<T, DP>(df, static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i, len, p.dh, lane);
+    own_rows<T, KD>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
+    own_rows<T, KD>(df, static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i, len, p.dh, lane);
     float delta = 0.f, lse = INFINITY;
     {
         // with o as it was rounded, D's error is the same for all of a row's keys and reaches dq and dk whole: as much again as
         // the rounding of dS where a row sees few keys
         const long row = ((long)b * p.N * p.Hq + h) * p.dh;
         Frag<T> of[KD], lo[KD];
-        own_rows<T, DP>(of, static_cast<const T*>(p.o) + row, (long)p.Hq * p.dh, i, len, p.dh, lane);
-        if (sizeof(T) == 2 && p.o_lo) own_rows<T, DP>(lo, static_cast<const T*>(p.o_lo) + row, (long)p.Hq * p.dh, i, len, p.dh, lane);
+        own_rows<T, KD>(of, static_cast<const T*>(p.o) + row, (long)p.Hq * p.dh, i, len, p.dh, lane);
+        if (sizeof(T) == 2 && p.o_lo) own_rows<T, KD>(lo, static_cast<const T*>(p.o_lo) + row, (long)p.Hq * p.dh, i, len, p.dh, lane);
 #pragma unroll
         for (int kk = 0; kk < KD; ++kk)
 #pragma unroll
@@ -651,10 +653,11 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
 // every head of the group.  KS waves share 32 keys, each with its own part of every query tile.  SINK: the 32 keys of a sinks'
 // tile and a share of ALL the query tiles, each wave's sums out in fp32 (window_sink_sum_kernel adds the shares in order).
-template <typename T, int DP, int NW, int KS, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
+template <typename T, int HW, int NW, int KS, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
+    constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
     using C = WCfg<T, DP>;
-    constexpr int NT = 64 * NW, RG = NW / KS, NS = BQ / 32 / KS, KD = DP / 16, ND = DP / 32, TILE = BQ * DP;
+    constexpr int NT = 64 * NW, RG = NW / KS, NS = BQ / 32 / KS, KD = HW / 16, ND = DP / 32, TILE = BQ * DP;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* lds = reinterpret_cast<T*>(smem);                 // two buffers of (Q tile, dO tile), then of BQ (lse, D) each
     float* stat = reinterpret_cast<float*>(lds + 4 * TILE);
@@ -686,9 +689,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
 
     Frag<T> kf[KD], vf[VLDS ? 1 : KD];
     T* Vs = reinterpret_cast<T*>(stat + 4 * BQ);         // VLDS: the workgroup's V rows stay in LDS
-    own_rows<T, DP>(kf, static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh, p.k.sn, j, len, p.dh, lane);
+    own_rows<T, KD>(kf, static_cast<const T*>(p.k.p) + (long)b * p.k.sb + (long)hk * p.k.sh, p.k.sn, j, len, p.dh, lane);
     const T* V = static_cast<const T*>(p.v.p) + (long)b * p.v.sb + (long)hk * p.v.sh;
-    if constexpr (!VLDS) own_rows<T, DP>(vf, V, p.v.sn, j, len, p.dh, lane);
+    if constexpr (!VLDS) own_rows<T, KD>(vf, V, p.v.sn, j, len, p.dh, lane);
 
     // queries that see key j: i - ilo <= span (unsigned); none for a key past the end
     int ilo = 1 << 30;
@@ -880,6 +883,7 @@ namespace {
 
 struct Plan {                  // tiles of one call
     int dp;                    // staged head width: 32, 64, 96 or 128
+    int width;                 // the width that the products over head elements take: dp, or 80 (in steps of 16)
     bool halves_q, halves_k;   // workgroups of 64 queries / keys whose rows are shared by two waves each, else of 128
     int sink_keys;             // keys that the sinks' launch takes (a multiple of 32, 0: none)
     int chunks, per_chunk;     // workgroups a sinks' tile, query tiles each of them takes
@@ -902,6 +906,8 @@ long halves_up_to(int dtype, int dp, bool uneven) { return dtype == VITK_F32 ? (
 Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bool causal, bool uneven) {
     Plan pl;
     pl.dp = (dh + 31) / 32 * 32;
+    pl.width = dh > 64 && dh <= 80 ? 80 : pl.dp;         // (4 x 1001 x 16 heads of 80, fp32: 196 + 696 us
+                                                         // forward and backward; as 96, a sixth more steps, 210 + 755; bf16 40 + 110, 41 + 114)
     // P and dS are rounded to bf16 for their products, an error of the size of the results' own rounding as long as many share in
     // it.  In a call of few scores single ones can carry dq and dk (up to 87 tokens, window 2: 0.0021 of the norm before the
     // result's own rounding, 0.0017 in large calls): there what the rounding took is multiplied too, in the forward as well,
@@ -987,36 +993,37 @@ template <typename T, int DP> size_t rows_lds(int groups, int n) {
     const size_t rows = 32 * groups * WCfg<T, DP>::LD * sizeof(T), join = n ? (size_t)groups * (DP / 2 * n + 2) * 64 * sizeof(float) : 0;
     return rows > join ? rows : join;
 }
-template <typename T, int DP, int KS, int BK, bool FINE = false> void run_fwd_tiles(WindowParams p, hipStream_t st) {
-    constexpr int WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;             // one wave a SIMD where two would spill
+template <typename T, int HW, int KS, int BK, bool FINE = false> void run_fwd_tiles(WindowParams p, hipStream_t st) {
+    constexpr int DP = (HW + 31) / 32 * 32, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;             // one wave a SIMD where two would spill
     p.tiles = (p.N + 32 * RG - 1) / (32 * RG);
     const unsigned grid = xcd_grid(p, p.tiles, p.G, by_tile(p));
     const size_t lds = std::max<size_t>(4 * BK * DP * sizeof(T), rows_lds<T, DP>(RG, KS - 1));
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, DP, NW, KS, BK, WPE, FINE>), lds);
-    hipLaunchKernelGGL((window_fwd_kernel<T, DP, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_fwd_kernel<T, HW, NW, KS, BK, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_fwd_kernel<T, HW, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
 // Key tiles of 64 in bf16; of 32 where the window is narrow and a tile of 64 would be mostly edge (16 x 577 tokens x 12 heads of
 // 64, window 64 on both sides: 24.1 us against 27.1, window 256: 33.5 against 34.7; 2 x 8192 x 16 heads of 128, causal window
 // of 512: 124.4 against 123.0, 16384 x 16, of 1024: 222 against 190).
-template <typename T, int DP> void run_fwd(const WindowParams& p, const Plan& pl, hipStream_t st) {
+template <typename T, int HW> void run_fwd(const WindowParams& p, const Plan& pl, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        if (pl.fine) return run_fwd_tiles<T, DP, 2, 64, true>(p, st);
+        if (pl.fine) return run_fwd_tiles<T, HW, 2, 64, true>(p, st);
     }
-    if (pl.halves_q) return run_fwd_tiles<T, DP, 2, 64>(p, st);
+    if (pl.halves_q) return run_fwd_tiles<T, HW, 2, 64>(p, st);
     if constexpr (sizeof(T) == 2) {
-        if (p.w < 0 || p.w > NARROW) return run_fwd_tiles<T, DP, 1, 64>(p, st);
+        if (p.w < 0 || p.w > NARROW) return run_fwd_tiles<T, HW, 1, 64>(p, st);
     }
-    run_fwd_tiles<T, DP, 1, 32>(p, st);
+    run_fwd_tiles<T, HW, 1, 32>(p, st);
 }
-template <typename T, int DP, int KS, bool FINE> void run_dq(WindowParams p, hipStream_t st) {
-    constexpr int BK = 32 * KS, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;
+template <typename T, int HW, int KS, bool FINE> void run_dq(WindowParams p, hipStream_t st) {
+    constexpr int DP = (HW + 31) / 32 * 32, BK = 32 * KS, WPE = sizeof(T) == 4 && DP == 128 ? 1 : 2, RG = NW / KS;
     p.tiles = (p.N + 32 * RG - 1) / (32 * RG);
     const unsigned grid = xcd_grid(p, p.tiles, p.G, by_tile(p));
     const size_t lds = std::max<size_t>(4 * BK * DP * sizeof(T), rows_lds<T, DP>(RG, KS - 1));
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, DP, NW, KS, BK, WPE, FINE>), lds);
-    hipLaunchKernelGGL((window_dq_kernel<T, DP, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dq_kernel<T, HW, NW, KS, BK, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_dq_kernel<T, HW, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
-template <typename T, int DP, int W, int KS, int BQ, bool SINK, bool FINE> void run_dkv(WindowParams p, int keys, hipStream_t st) {
+template <typename T, int HW, int W, int KS, int BQ, bool SINK, bool FINE> void run_dkv(WindowParams p, int keys, hipStream_t st) {
+    constexpr int DP = (HW + 31) / 32 * 32;
     // V rows in LDS where they, K's and both accumulators do not fit the registers of two waves a SIMD
     constexpr bool VLDS = sizeof(T) == 2 && DP >= 96 && !SINK;
     constexpr int WPE = (sizeof(T) == 4 && DP >= 96) || SINK || (FINE && DP == 128) ? 1 : 2, RG = W / KS;
@@ -1026,23 +1033,23 @@ template <typename T, int DP, int W, int KS, int BQ, bool SINK, bool FINE> void 
     const unsigned grid = xcd_grid(p, p.tiles - p.heavy, SINK ? p.chunks : 1, !SINK && by_tile(p)) + (p.heavy * p.B * p.Hk + 7) / 8 * 8;
     const size_t tl = 4 * BQ * DP * sizeof(T) + 4 * BQ * sizeof(float) + (VLDS ? 32 * RG * DP * sizeof(T) : 0);
     const size_t lds = std::max<size_t>(tl, rows_lds<T, DP>(RG, 2 * (KS - 1)));
-    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, DP, W, KS, BQ, SINK, VLDS, WPE, FINE>), lds);
-    hipLaunchKernelGGL((window_dkv_kernel<T, DP, W, KS, BQ, SINK, VLDS, WPE, FINE>), dim3(grid), dim3(64 * W), lds, st, p);
+    vitk_lds_optin(reinterpret_cast<const void*>(&window_dkv_kernel<T, HW, W, KS, BQ, SINK, VLDS, WPE, FINE>), lds);
+    hipLaunchKernelGGL((window_dkv_kernel<T, HW, W, KS, BQ, SINK, VLDS, WPE, FINE>), dim3(grid), dim3(64 * W), lds, st, p);
 }
-template <typename T, int DP, bool FINE> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
-    constexpr int BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
+template <typename T, int HW, bool FINE> void run_bwd(WindowParams p, const Plan& pl, void* dq, hipStream_t st) {
+    constexpr int DP = (HW + 31) / 32 * 32, BQ = sizeof(T) == 2 && DP <= 64 ? 64 : 32;
     p.out = dq;
     if constexpr (!FINE) {
-        if (!pl.halves_q) run_dq<T, DP, 1, FINE>(p, st);
+        if (!pl.halves_q) run_dq<T, HW, 1, FINE>(p, st);
     }
-    if (pl.halves_q) run_dq<T, DP, 2, FINE>(p, st);
+    if (pl.halves_q) run_dq<T, HW, 2, FINE>(p, st);
     if (pl.sink_keys) {
         WindowParams s = p;
         s.key0 = 0;
         s.chunks = pl.chunks;
         s.per_chunk = pl.per_chunk;
         constexpr int W = sink_waves(DP * sizeof(T));
-        run_dkv<T, DP, W, W, 32 * W, true, FINE>(s, pl.sink_keys, st);
+        run_dkv<T, HW, W, W, 32 * W, true, FINE>(s, pl.sink_keys, st);
         s.tiles = pl.sink_keys / 32;
         s.chunks = pl.shares;
         hipLaunchKernelGGL((window_sink_sum_kernel<T, DP>), dim3((unsigned)((long)p.B * p.Hk * s.tiles * 2 * (DP / 2))), dim3(256),
@@ -1052,15 +1059,15 @@ template <typename T, int DP, bool FINE> void run_bwd(WindowParams p, const Plan
     const int rest = p.N - pl.sink_keys;
     if (rest <= 0) return;
     if constexpr (!FINE) {
-        if (!pl.halves_k) run_dkv<T, DP, NW, 1, BQ, false, FINE>(p, rest, st);
+        if (!pl.halves_k) run_dkv<T, HW, NW, 1, BQ, false, FINE>(p, rest, st);
     }
-    if (pl.halves_k) run_dkv<T, DP, NW, 2, 64, false, FINE>(p, rest, st);
+    if (pl.halves_k) run_dkv<T, HW, NW, 2, 64, false, FINE>(p, rest, st);
 }
-template <typename T, int DP> void run_bwd(const WindowParams& p, const Plan& pl, void* dq, hipStream_t st) {
+template <typename T, int HW> void run_bwd(const WindowParams& p, const Plan& pl, void* dq, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        if (pl.fine) return run_bwd<T, DP, true>(p, pl, dq, st);
+        if (pl.fine) return run_bwd<T, HW, true>(p, pl, dq, st);
     }
-    run_bwd<T, DP, false>(p, pl, dq, st);
+    run_bwd<T, HW, false>(p, pl, dq, st);
 }
 
 }  // namespace
@@ -1088,9 +1095,10 @@ extern "C" int vitk_window_attn_fwd(int dtype, int B, int N, int Hq, int Hk, int
     p.lse = lse;
     const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal, p.causal || p.w >= 0 || lengths);
 #define GO(T, D) run_fwd<T, D>(p, pl, stream)
-#define BY_DP(T) switch (pl.dp) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 96: GO(T, 96); break; default: GO(T, 128); break; }
-    if (dtype == VITK_BF16) { BY_DP(__bf16) }
-    else { BY_DP(float) }
+#define BY_WIDTH(T) switch (pl.width) { case 32: GO(T, 32); break; case 64: GO(T, 64); break; case 80: GO(T, 80); break; \
+                                       case 96: GO(T, 96); break; default: GO(T, 128); break; }
+    if (dtype == VITK_BF16) { BY_WIDTH(__bf16) }
+    else { BY_WIDTH(float) }
 #undef GO
     VITK_CHECK_LAUNCH(what);
     return VITK_OK;
@@ -1138,10 +1146,10 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     p.dv = dv;
     const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal, p.causal || p.w >= 0 || lengths);
 #define GO(T, D) run_bwd<T, D>(p, pl, dq, stream)
-    if (dtype == VITK_BF16) { BY_DP(__bf16) }
-    else { BY_DP(float) }
+    if (dtype == VITK_BF16) { BY_WIDTH(__bf16) }
+    else { BY_WIDTH(float) }
 #undef GO
-#undef BY_DP
+#undef BY_WIDTH
     VITK_CHECK_LAUNCH(what);
     return VITK_OK;
 }
