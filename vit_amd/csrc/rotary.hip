@@ -139,7 +139,8 @@ struct RotaryParams {
 };
 
 // A lane keeps its unit's turn in registers and applies it to HPT heads of the token, all of whose loads are in flight
-// at once.
+// at once.  32 x 577 x 12 heads of 64, bf16: 11.7 us for 57 MB (out of the last-level cache); 16411 x 16 heads of 80, fp32, half of
+// it turned: 44 us for 169 MB, 3.8 TB/s, where a copy of 4 GiB does 4.8.
 template <typename T, int V, bool INTER, int HPT>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
     const unsigned id = blockIdx.x * 256u + threadIdx.x;
@@ -224,7 +225,9 @@ __device__ __forceinline__ float row_sum(float v, int lpr_log2) {
 // One row (token, head) on 2^lpr_log2 lanes, 256 >> lpr_log2 of them side by side in a workgroup; a lane group takes HPT
 // heads of one token in a step, so that the token's turn, 8 bytes a pair against 4 or 8 of x, is read once for HPT rows.
 // BWD walks several steps per workgroup so that gamma's sum stays in registers and ends in one partial row per workgroup (a
-// second kernel adds those in a fixed order: no atomics).
+// second kernel adds those in a fixed order: no atomics).  128 x 197 x (12 + 12) heads of 64, bf16: forward 31 us, backward 58 +
+// 6, for 155 and 232 MB (5.0 and 4.0 TB/s); 32769 x (16 + 4) heads of 80, fp32: 87 us, 130 + 7, for 419 and 629 MB (4.8 TB/s, a large
+// copy's rate).
 template <typename T, int V, bool INTER, int HPT, bool BWD>
 __global__ __launch_bounds__(256) void qk_norm_kernel(const QkNormParams p) {
     const bool isq = blockIdx.x < p.q.blocks;

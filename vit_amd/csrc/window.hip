@@ -11,7 +11,8 @@
 // O^T += V^T P^T (the order of the contraction's 16 keys is the accumulator's own; V^T fragments come from the row-major
 // V tile in LDS by transpose reads in that same order).  Nothing of size N x N exists and nothing is summed by atomics:
 // the backward makes the scores twice (queries' kernel, keys' kernel).  Sums, maxima and the softmax are fp32; with bf16
-// inputs P and dS are rounded to bf16 as operands of their MFMA, each once.
+// inputs P and dS are rounded to bf16 as operands of their MFMA, each once; in calls of few scores what that took is
+// multiplied as well.
 #include <algorithm>
 #include "common.h"
 
@@ -321,7 +322,13 @@ template <int ND> __device__ __forceinline__ void half_add(const float* x, f32x1
 }
 
 // ---------------------------------------------------------------------------------------------------------- forward
-// A wave owns 32 queries; KS = 2: two waves share them, each with one half of every tile of keys.
+// A wave owns 32 queries; KS = 2: two waves share them, each with one half of every tile of keys.  HW: head width in steps of 16.
+// Tiles come by asynchronous loads into one of two images while the other is used, one barrier a tile.  Bound by the matrix
+// unit and the softmax's vector work in turn (32 exponentials, maxima, sums and conversions of them beside 32 MFMA a wave and
+// tile of 64 keys of 128): two waves a SIMD cover each other's, and no part taken out by itself gives more than 15 %.
+// bf16, heads of 128: 8192 tokens x 16 heads, causal, 290 us = 950 TFLOP/s of visible pairs; 16384 tokens with a causal window
+// of 1024 181 us = 740, a ninth of whose pairs are the window's and the diagonal's edges and are thrown away.  fp32, heads of 80:
+// 4 x 1001 x 16 196 us = 105 TFLOP/s of 154.
 template <typename T, int HW, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowParams p) {
     constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
@@ -523,6 +530,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
 }
 
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
+// The forward's walk with three products (S, dP, dS K); 270 us = 740 TFLOP/s at the forward's windowed size.
 template <typename T, int HW, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowParams p) {
     constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
@@ -653,6 +661,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
 // every head of the group.  KS waves share 32 keys, each with its own part of every query tile.  SINK: the 32 keys of a sinks'
 // tile and a share of ALL the query tiles, each wave's sums out in fp32 (window_sink_sum_kernel adds the shares in order).
+// Four products (S, dP, P dO, dS Q) on the same two operands: 300 us = 890 TFLOP/s at the forward's windowed size.
 template <typename T, int HW, int NW, int KS, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
     constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
@@ -897,7 +906,7 @@ constexpr int NARROW = 256;
 
 // Up to how many workgroups of 128 rows there are, that workgroups of 64 with two waves a row, each with half of the other axis,
 // are faster.  One of 128 takes as long as its longest row, whatever the other CUs do: few of them leave CUs, and a second
-// round of them most of its CUs, waiting.  Halves read every tile for half the rows.  fp32, 16 heads x 1001 tokens of 80, forward
+// round of them most of its CUs, waiting.  Halves read every tile for half the rows.  fp32, 16 heads x 1001 tokens of 80 (as 96), forward
 // and backward: one sequence 68 + 205 us against 120 + 390, three 200 + 608 against 209 + 749, four 265 + 808 against 211 +
 // 759; causal, four of 1024: 201 + 605 against 210 + 746.  bf16, 16 x 1024: heads of 128 24 + 59 against 31 + 93, two sequences
 // 31 + 99 against 34 + 95, three 47 + 149 against 41 + 118; of 64 three 26 + 75 against 28 + 76, four 33 + 92 against 30 + 83.
@@ -917,10 +926,12 @@ Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bo
     pl.fine = dtype == VITK_BF16 && (long)B * Hq * N * keys <= FINE;
     const long tq = (long)B * Hq * ((N + 127) / 128), tk = (long)B * Hk * ((N + 127) / 128), most = halves_up_to(dtype, pl.dp, uneven);
     pl.halves_q = pl.fine || tq <= most;
-    pl.halves_k = pl.fine || tk <= most;
+    // (causal without a window: the first keys' rows are twice the average, times the group's heads.  8 ragged sequences up to 1500
+    // x 16 heads of 80 in groups of 4: the backward 202 us against 303; 2 x 8192 x 12 of 64 in groups of 3: 879 against 996)
+    pl.halves_k = pl.fine || tk <= (dtype == VITK_BF16 && causal && w < 0 ? 2 * most : most);
     // The sinks' keys are seen by all N queries, the 128 of another tile by `near` of them.  Where that is over four times more, or
     // so much that the ordinary launch would wait for the sinks' tiles, they get a launch of their own, whose workgroups share
-    // the queries, and a sum; else they go first in the ordinary one (16 x 577 tokens x 12 heads, window 64: 39 us in all
+    // the queries, and a sum; else they go first in the ordinary one (16 x 577 tokens x 12 heads, window 64: 37 us in all
     // against 33 + 14 + 7; backward of 1 x 577 x 12: 26 against 31, of 1001 tokens x 8 heads in groups of 4, causal window of
     // 100: 85 against 44, fp32 314 against 125).
     const long near = 128 + (causal ? 1L : 2L) * w;
@@ -974,18 +985,23 @@ void fill_params(WindowParams& p, int B, int N, int Hq, int Hk, int dh, int w, i
 // ones first, dealt to the XCDs in turn: where pieces differ (sequences of different lengths, causal rows without a window:
 // 8192 tokens x 16 heads of 128, groups of 4, forward and backward 290 + 1214 us; in runs of 16 to each XCD, some of which then
 // had all the long ones, 405 + 2147), and where heads are a multiple of 8, so that a head stays on one XCD (16 x 577 x 12 heads
-// of 64, window 64: 20 + 62 us against 22 + 66).  Else an eighth of the pieces in a row to each XCD (16384 tokens, groups of 4
-// heads of 128, window 1024: 181 + 555 us against 183 + 567).
+// of 64, window 64: 20 + 62 us against 22 + 66).  A multiple of 8 heads whose tiles differ by the sequence alone: whole heads to
+// each XCD in turn (1001, 100 and 1001 tokens x 16 heads of 80, fp32: 138 + 411 us against 188 + 559 by tile).  Else an eighth of
+// the pieces in a row to each XCD (16384 tokens, groups of 4 heads of 128, window 1024: 181 + 555 us against 183 + 567).
 unsigned xcd_grid(WindowParams& p, int tiles, int each, bool by_tile) {
     const int heads = p.B * p.Hk, total = heads * tiles * each;
     p.total = total;
     p.by_tile = by_tile;
     p.inner = by_tile ? heads : tiles;
-    p.run = by_tile ? each : (total + 7) / 8;
+    p.run = by_tile ? each : (p.lengths && heads % 8 == 0 ? tiles * each : (total + 7) / 8);
     const long round = 8L * p.run;
     return (unsigned)((total + round - 1) / round * round);
 }
-bool by_tile(const WindowParams& p) { return p.lengths || (p.causal && p.w < 0) || (long)p.B * p.Hk % 8 == 0; }
+bool by_tile(const WindowParams& p) {
+    const bool eights = (long)p.B * p.Hk % 8 == 0;
+    if (p.w < 0 && !p.causal && p.lengths && eights) return false;
+    return p.lengths || (p.causal && p.w < 0) || eights;
+}
 
 constexpr int NW = 4;
 // bytes of LDS that `waves` groups of 32 rows need to leave through (put_rows), after which `n` accumulators of theirs were joined

@@ -1182,7 +1182,8 @@ def window_attention(q, k, v, window, sinks=0, causal=False, scale=None, lengths
     query i sees the keys j with |i - j| <= window, and the first ``sinks`` keys (class / register tokens) wherever it is;
     ``causal``: of those only j <= i.  window < 0: every key.  ``lengths`` (int32 [B]): tokens of each padded sequence; rows past
     it are not read, and their outputs and gradients are 0.  scale: dh^-0.5 unless given (positive).  out [B, N, Hq, dh],
-    contiguous."""
+    contiguous.  Non-finite values reach the outputs of the rows that see them and no others; in the backward also the gradients
+    of rows and keys around them."""
     return WindowAttentionFn.apply(q, k, v, window, sinks, causal, q.shape[-1] ** -0.5 if scale is None else scale, lengths)
 
 
