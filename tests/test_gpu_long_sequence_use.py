@@ -196,3 +196,26 @@ def test_sinks_of_their_own_launch(case, dtype):
         want = R.window_attention(q, k, v, window, sinks, causal, dh ** -0.5, n, do)
         for t, x in got.items():
             R.within(x, *want[t], t)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('case', [
+    # B, N, Hq, Hk, dh, window, sinks, causal, padded: workgroups of 128 rows at every width, every order of the work
+    (9, 1030, 8, 8, 32, 200, 5, False, False), (9, 1030, 8, 8, 80, 300, 3, True, False), (9, 1030, 7, 7, 80, -1, 0, False, False),
+    (9, 1030, 8, 8, 96, 30, 4, True, False), (9, 1030, 8, 8, 48, -1, 0, False, True), (9, 1030, 8, 8, 112, -1, 0, True, True),
+    (11, 1030, 7, 7, 64, 260, 40, False, True), (5, 1030, 16, 2, 72, -1, 0, True, False), (5, 1030, 16, 4, 128, 400, 130, True, False),
+    (40, 200, 14, 7, 64, 20, 1, False, True), (1, 4100, 18, 18, 64, 70, 3, True, False)], ids=str)
+def test_large_calls(case, dtype):
+    from vit_amd import functional as VF
+    B, N, Hq, Hk, dh, window, sinks, causal, padded = case
+    g = _gen(49)
+    q, k, v, do = (torch.randn(B, N, h, dh, generator=g, device='cuda').to(dtype) for h in (Hq, Hk, Hk, Hq))
+    n = torch.randint(0, N + 1, (B,), generator=g, device='cuda', dtype=torch.int32) if padded else None
+    ins = [t.requires_grad_(True) for t in (q, k, v)]
+    o = VF.window_attention(*ins, window, sinks=sinks, causal=causal, lengths=n)
+    got = dict(zip(('o', 'dq', 'dk', 'dv'), (o.detach(), *torch.autograd.grad(o, ins, do))))
+    want = R.window_attention(*(t.detach() for t in ins), window, sinks, causal, dh ** -0.5, n, do)
+    for t, x in got.items():
+        R.within(x, *want[t], t)
+    again = torch.autograd.grad(VF.window_attention(*ins, window, sinks=sinks, causal=causal, lengths=n), ins, do)
+    assert all(torch.equal(a, got[t]) for a, t in zip(again, ('dq', 'dk', 'dv')))
