@@ -219,3 +219,23 @@ def test_large_calls(case, dtype):
         R.within(x, *want[t], t)
     again = torch.autograd.grad(VF.window_attention(*ins, window, sinks=sinks, causal=causal, lengths=n), ins, do)
     assert all(torch.equal(a, got[t]) for a, t in zip(again, ('dq', 'dk', 'dv')))
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('N', [40, 600])
+@pytest.mark.parametrize('window', [-1, 9])
+def test_infinite_values(N, window, dtype):
+    """An infinite value makes the rows that see it infinite in its element, with its sign, and leaves the others alone."""
+    from vit_amd import functional as VF
+    g = _gen(50)
+    q, k, v = (torch.randn(2, N, 2, 64, generator=g, device='cuda').to(dtype) for _ in range(3))
+    want, bound = R.window_attention(q, k, v, window, 0, False, 0.125, None)['o']
+    v[0, 21, 1, 5], v[1, 30, 0, 63] = float('inf'), float('-inf')
+    o = VF.window_attention(q, k, v, window)
+    i = torch.arange(N, device='cuda')
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    for b, j, h, d, sign in ((0, 21, 1, 5, 1.0), (1, 30, 0, 63, -1.0)):
+        seen = (i - j).abs() <= (window if window >= 0 else N)
+        assert (o[b, seen, h, d] == sign * float('inf')).all()
+        hit[b, seen, h, d] = True
+    R.within(o[~hit], want[~hit], bound[~hit], 'others')

@@ -478,13 +478,14 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     }
     const bool none = i >= len || (m == -INFINITY && l == 0.f);      // nothing visible (a NaN sum stays a NaN)
     // A non-finite V of a key that only some queries of a tile see has reached the others as 0 * V.  Where the result is not
-    // finite, it is made again key by key, for the keys that each query sees.
+    // finite, it is made again key by key, for the keys that each query sees.  (FINE: p and its remainder can be of two signs,
+    // and infinity times both is no number.)
     float bad = 0.f;
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) bad += o[t][e] * 0.f;
-    if ((p.w >= 0 || p.causal) && __any(!none && bad != 0.f && l == l)) {         // (a NaN is unequal; a NaN sum is the row's own)
+    if ((FINE || p.w >= 0 || p.causal) && __any(!none && bad != 0.f && l == l)) {         // (a NaN is unequal; a NaN sum is the row's own)
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
