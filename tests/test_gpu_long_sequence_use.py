@@ -239,3 +239,21 @@ def test_infinite_values(N, window, dtype):
         assert (o[b, seen, h, d] == sign * float('inf')).all()
         hit[b, seen, h, d] = True
     R.within(o[~hit], want[~hit], bound[~hit], 'others')
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=['f32', 'bf16'])
+@pytest.mark.parametrize('B,N,H,dh', [(4, 1, 8, 80), (2, 5, 2, 64), (1, 300, 4, 128), (9, 1030, 8, 32), (16, 1, 3, 24)])
+def test_rows_that_see_themselves_alone(B, N, H, dh, dtype):
+    """The softmax of one score is 1 whatever the score: dq is exactly 0, and so is dk where every row is like that."""
+    from vit_amd import functional as VF
+    g = _gen(51)
+    q, k, v, do = (torch.randn(B, N, h, dh, generator=g, device='cuda').to(dtype) for h in (2 * H, H, H, 2 * H))
+    ins = [t.requires_grad_(True) for t in (q, k, v)]
+    dq, dk, _ = torch.autograd.grad(VF.window_attention(*ins, 0), ins, do)
+    assert not dq.any() and not dk.any()
+    for window, sinks, lengths in ((-1, 0, None), (3, 2, torch.ones(B, dtype=torch.int32, device='cuda'))):
+        dq, dk, _ = torch.autograd.grad(VF.window_attention(*ins, window, sinks=sinks, causal=True, lengths=lengths), ins, do)
+        assert not dq[:, 0].any()
+        assert lengths is None or not (dq.any() or dk.any())
+    dq, _, _ = torch.autograd.grad(VF.window_attention(*ins, 0, sinks=1, causal=True), ins, do)
+    assert not dq[:, 0].any() and (N == 1 or dq[:, 1:].any(-1).all())

@@ -272,6 +272,11 @@ __device__ __forceinline__ RowRange row_range(const WindowParams& p, int i, int 
     r.s = min(p.S, e + 1);
     return r;
 }
+constexpr int ALONE = (1 << 30) + 1;                     // RowRange::lo of such a row in the backward, past every key
+__device__ __forceinline__ bool sees_itself_alone(const RowRange& r) {      // (a row within the length always sees itself)
+    const int lo = max(r.lo, 0), hi = r.lo + (int)r.span;
+    return lo == hi && min(r.s, lo) == 0 && r.s <= hi + 1;         // no sink before or behind its window
+}
 // What a wave's queries [i, i + BQ) see of keys [j0, j0 + BK): NOTHING, ALL, or which of its edges the test has to look at
 enum { NOTHING = 0, ALL = 1, EDGE_HI = 2, EDGE_LO = 4, EDGE_ANY = 8 };
 __device__ __forceinline__ int tile_kind(const WindowParams& p, int i, int BQ, int j0, int BK, int len) {
@@ -556,6 +561,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
     Frag<T> qf[KD], df[KD];
     own_rows<T, KD>(qf, static_cast<const T*>(p.q.p) + (long)b * p.q.sb + (long)h * p.q.sh, p.q.sn, i, len, p.dh, lane);
     own_rows<T, KD>(df, static_cast<const T*>(p.dout.p) + (long)b * p.dout.sb + (long)h * p.dout.sh, p.dout.sn, i, len, p.dh, lane);
+    // a row that sees nothing but its own key has dS = 0, and exactly so: D is what the products make of do . v, dP's own bits
+    RowRange rr = row_range(p, i, len);
+    if (i < len && sees_itself_alone(rr)) rr = RowRange{ALONE, 0u, 0};
     float delta = 0.f, lse = INFINITY;
     {
         // with o as it was rounded, D's error is the same for all of a row's keys and reaches dq and dk whole: as much again as
@@ -574,10 +582,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
         delta = half_sum(delta);
         const long at = ((long)b * p.Hq + h) * p.N + i;
         if (i < len) lse = p.lse[at];
-        if (!part && lane < 32 && i < p.N) p.delta[at] = delta;
+        if (!part && rr.lo != ALONE && lane < 32 && i < p.N) p.delta[at] = delta;
     }
     const KeyTiles kt = key_tiles(p, i0, i0 + 32 * RG, len, BK);
-    const RowRange rr = row_range(p, i, len);
     f32x16 dq[ND];
 #pragma unroll
     for (int t = 0; t < ND; ++t)
@@ -618,6 +625,13 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
                     s = mma32(a, qf[kk], s);
                     row_frag32<DP>(a, Vs, 32 * u, kk, lane);
                     dp = mma32(a, df[kk], dp);
+                }
+                if (j0 + 32 * u == iw && __any(rr.lo == ALONE)) {
+                    float own = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) own = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31) ? dp[e] : own;
+                    own = half_sum(own);
+                    if (rr.lo == ALONE && lane < 32) p.delta[((long)b * p.Hq + h) * p.N + i] = own;
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.sc2, -lse)) * (dp[e] - delta);
