@@ -541,8 +541,11 @@ def _aligned_heads(t):
     """16-byte aligned rows, neighbours of a sequence under 16 MiB apart, as the attention kernels read them: ``t`` itself, or a
     copy."""
     es, s = t.element_size(), t.stride()
-    per = 16 // es
-    if s[-1] == 1 and t.data_ptr() % 16 == 0 and not any(x % per for x in s[:-1]) and (len(s) < 4 or s[1] * es < 1 << 24):
+    n = len(s)
+    if n not in (3, 4):                                  # refused by its caller's checks
+        return t
+    if s[-1] == 1 and t.data_ptr() % 16 == 0 and (s[0] | s[1] | (s[2] if n == 4 else 0)) * es % 16 == 0 and \
+            (n == 3 or s[1] * es < 1 << 24):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
