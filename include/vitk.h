@@ -299,7 +299,8 @@ int vitk_qk_norm_rotary_bwd(int dtype, int interleaved, int B, int N, int Hq, in
 /* Attention of query i over the keys j with |i - j| <= window, and the first `sinks` keys always (causal: only j <= i);
  * window < 0: every key.  Query head h reads key head h / (Hq / Hk).  lengths (int32 [B], may be NULL): tokens of each padded
  * sequence; rows past it are not read, their outputs and gradients are 0.  dh: a multiple of 8 up to 128; pointers and strides
- * 16-byte aligned, neighbouring tokens of q, k, v and dout under 16 MiB apart.  lse [B][Hq][N] fp32 (may be NULL in a forward without backward): log2 of the softmax sum, +inf for a row that
+ * 16-byte aligned, neighbouring tokens of q, k, v and dout under 16 MiB apart (on the same memory, too: stride 0, or less than
+ * dh).  lse [B][Hq][N] fp32 (may be NULL in a forward without backward): log2 of the softmax sum, +inf for a row that
  * sees nothing (its output is 0).  out_lo (bf16, like out, may be NULL): what the rounding took from out, for the backward of
  * the same call (which then has o . do to 2^-16).  The backward sums nothing with atomics.  Forward: a row depends on nothing
  * that it does not see, NaN and infinities included; backward: a non-finite value of a token within the lengths can reach the

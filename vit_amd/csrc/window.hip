@@ -145,9 +145,11 @@ template <int BYTES> __device__ __forceinline__ void load_to_lds(const void* bas
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }     // vmcnt(0), in a form the compiler counts
 
 // Rows [row0, row0 + ROWS) of a strided matrix into an image, asynchronously and without passing through registers; rows outside
-// [0, hi) and columns >= dh are zero.  The bounds are the buffer descriptor's (what lies outside reads as zero), and the
-// descriptor is moved to every tile's first row, so offsets in it stay small however long the sequence is.  The data is
-// there after the next tile_ready().
+// [0, hi) and columns >= dh are zero, but for rows that share memory (sn < dh: a gradient broadcast over the tokens comes with
+// sn = 0): what lies behind their last row are other rows' elements, and a reader masks it.  (Zeros there too, by a branch for the
+// last tile of such rows: 5 % of the backward at 64 wide heads.)  The bounds are the buffer descriptor's (what lies outside reads as
+// zero), and the descriptor is moved to every tile's first row, so offsets in it stay small however long the sequence is.
+// The data is there after the next tile_ready().
 template <typename T, int DP, int ROWS, int NT> struct Stager {
     using C = WCfg<T, DP>;
     static constexpr int LOADS = ROWS * C::CPR / 64, CH = (LOADS + NT / 64 - 1) / (NT / 64);    // of the workgroup, of a wave
@@ -484,13 +486,13 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     const bool none = i >= len || (m == -INFINITY && l == 0.f);      // nothing visible (a NaN sum stays a NaN)
     // A non-finite V of a key that only some queries of a tile see has reached the others as 0 * V.  Where the result is not
     // finite, it is made again key by key, for the keys that each query sees.  (FINE: p and its remainder can be of two signs,
-    // and infinity times both is no number.)
+    // and infinity times both is no number.  V rows that share memory: so has what lies behind the last one.)
     float bad = 0.f;
 #pragma unroll
     for (int t = 0; t < ND; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) bad += o[t][e] * 0.f;
-    if ((FINE || p.w >= 0 || p.causal) && __any(!none && bad != 0.f && l == l)) {         // (a NaN is unequal; a NaN sum is the row's own)
+    if ((FINE || p.w >= 0 || p.causal || p.v.sn < p.dh) && __any(!none && bad != 0.f && l == l)) {         // (a NaN is unequal; a NaN sum is the row's own)
 #pragma unroll
         for (int t = 0; t < ND; ++t)
 #pragma unroll
@@ -754,7 +756,6 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
     Stager<T, DP, BQ, NT> sq, sd;
     sq.init(p.q.sn, p.dh);
     sd.init(p.dout.sn, p.dh);
-    // rows past the end come as zeros, statistics too: their p is 1 there, and meets zeros of dO, D and Q
     auto fetch = [&](int it) {
         const int gi = uniform(it / nt), h = hk * p.G + gi, i0 = BQ * (ta + it - gi * nt);
         T* nx = lds + (it & 1) * 2 * TILE;
@@ -834,7 +835,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         const int i0 = BQ * (ta + it - uniform(it / nt) * nt) + 32 * NS * part;
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
-            const int kind = jw < len ? tile_kind(p, i0 + 32 * u, 32, jw, 32, len) : 0;
+            int kind = jw < len ? tile_kind(p, i0 + 32 * u, 32, jw, 32, len) : 0;
+            // queries past the end: their statistics come as zeros, so p is 1 or more there, and dO's and Q's rows may be others'
+            if (kind && i0 + 32 * u + 32 > len) kind = EDGE_ANY;
             if (kind) tile(kind, Qs, Ds, ls, u, i0);
         }
     }
