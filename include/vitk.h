@@ -48,10 +48,9 @@ int vitk_get_reserved_cus(void);
  * library does that itself it launches a kernel of its own (vitk_zero_async in csrc/runtime.hip), never hipMemsetAsync.
  * Reason: with hipMemsetAsync nodes in a training step captured by torch.cuda.graph (ROCm 7.2, PyTorch 2.10), the
  * second replay accumulated onto stale data (logits 5e36); the same step with kernel zero fills replays bit-stably.
- * The cause was not isolated: tools/micro/memset_graph.hip captures hundreds of (memset, accumulate, check) triples
- * with plain HIP -- hipMemsetAsync on large, tiny and pitched targets, hipMemsetD32Async -- and every replay is correct, so
- * memset nodes as such are not broken; the failure needed the torch capture (its private memory pool and capture mode)
- * around ctypes calls.  A caller that captures these entry points and zeroes the accumulation targets itself should do it
+ * The cause was not isolated: a graph of hundreds of (memset, accumulate, check) triples captured with plain HIP --
+ * hipMemsetAsync on large, tiny and pitched targets, hipMemsetD32Async -- replayed correctly; the failure needed the torch
+ * capture (its private memory pool and capture mode) around ctypes calls.  A caller that captures these entry points and zeroes the accumulation targets itself should do it
  * with a kernel (torch's zero_() is one) rather than a memset node, or verify two replays against eager as
  * tests/test_gpu_graph.py does. */
 /* C = epilogue(alpha * op(A) op(B) + bias) [+ residual]      (MFMA, fp32 accumulate)

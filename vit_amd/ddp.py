@@ -36,8 +36,8 @@ def init_process_group(backend='nccl', device=None, **kw):
 
     Only for a process that has not run the fused blocks yet (the reference's order too: init_distributed_mode, then the
     model, train.py:631-635).  A high-priority RCCL stream made AFTER the process had trained on its main and side streams
-    left the next step's kernels pending for good (torch.cuda.synchronize() never returned; tools/diag_reducer_hang.py:
-    main stream, side stream and every bucket pending -- with a normal-priority RCCL stream the same sequence runs).  The
+    left the next step's kernels pending for good (torch.cuda.synchronize() never returned: main stream, side stream and
+    every bucket pending -- with a normal-priority RCCL stream the same sequence runs).  The
     cause inside the runtime is not known; such a process gets the normal class, and the side stream is chosen again so
     that the overlap probe sees the queues as they are now.  VITK_RCCL_HIGH_PRIORITY=0 / =1 forces either."""
     if backend == 'nccl':
