@@ -14,6 +14,7 @@
 // inputs P and dS are rounded to bf16 as operands of their MFMA, each once; in calls of few scores what that took is
 // multiplied as well.
 #include <algorithm>
+#include <type_traits>
 #include "common.h"
 
 namespace vitk {
@@ -105,6 +106,8 @@ struct WindowParams {
     void *out, *dk, *dv;          // out: o in the forward, dq in the queries' backward kernel; all [B][N][H][dh]
     float* lse;                   // [B][Hq][N]: log2 of the softmax sum, maximum included; +inf where a row sees nothing
     float* delta;                 // [B][Hq][N]: D_i, written by the queries' kernel for the keys' kernel
+    int* far;                     // the same way, [B][Hq][groups of 32 rows]: whether one of them has a far log-sum
+    float* shift;                 // [B][Hq][N]: in such groups, what the rows' exponents lack
     float* part;                  // sinks' partial sums [B*Hk][key tiles][chunks][dk, dv][DP][32] fp32
     const int* lengths;           // [B] or NULL
     int B, N, Hq, Hk, G, dh;
@@ -537,6 +540,19 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     if (sizeof(T) == 2 && p.o_lo) put_rows<T, DP, true>(o, 1.f / l, none, mine, static_cast<T*>(p.o_lo) + at, ldg, iw, p.N, p.dh, lane);
 }
 
+// The backward makes P again as exp2(score - lse), and lse's rounding is an error of its whole row: 2^-16 of P at most up to an
+// |lse| of FAR, but 2^-4 at a million, and past FAR_ROUNDED, where the forward rounds the products, a power of two of its own.
+// Where one of 32 rows is out there (a diverging model's), all of them take their scores minus lse for scores, with a log-sum of
+// 0, and have P's sum made again beside dq to divide by.  That is a second copy of the loops, which a workgroup takes if it
+// meets such rows: a test within the loops cost 4 to 8 % of the backward, this 0 to 2.
+constexpr float FAR = 512.f, FAR_ROUNDED = 16777216.f;
+__device__ __forceinline__ bool beyond(float lse, float limit) { return !(fabsf(lse) <= limit); }
+__device__ __forceinline__ float far_exponent(float s, float sc2, float lse, bool rounded) {
+    float x = s * sc2;
+    asm("" : "+v"(x));                                   // two roundings: not to be contracted
+    return rounded ? x - lse : fmaf(s, sc2, -lse);
+}
+
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
 // The forward's walk with three products (S, dP, dS K); 270 us = 740 TFLOP/s at the forward's windowed size.
 template <typename T, int HW, int NW, int KS, int BK, int WPE, bool FINE>
@@ -586,6 +602,15 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
         if (i < len) lse = p.lse[at];
         if (!part && rr.lo != ALONE && lane < 32 && i < p.N) p.delta[at] = delta;
     }
+    bool any_far = false;                                // the same for the whole workgroup
+#pragma unroll
+    for (int r = 0; r < 32 * RG; r += 64) {
+        const int row = i0 + r + lane;
+        any_far |= __any(row < len && beyond(p.lse[((long)b * p.Hq + h) * p.N + min(row, p.N - 1)], FAR)) != 0;
+    }
+    const bool far = __any(i < len && beyond(lse, FAR));
+    float total = 0.f;                                   // far: the sum of P over this lane's keys
+    if (!part && lane == 0 && iw < len) p.far[((long)b * p.Hq + h) * ((p.N + 31) / 32) + iw / 32] = far;
     const KeyTiles kt = key_tiles(p, i0, i0 + 32 * RG, len, BK);
     f32x16 dq[ND];
 #pragma unroll
@@ -602,75 +627,109 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
         sk.load(K, p.k.sn, j0, len, p.dh, lds, wave);
         sv.load(V, p.v.sn, j0, len, p.dh, lds + TILE, wave);
     }
-    for (int it = 0; it < kt.n; ++it) {
-        const T* Ks = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
-        const T* Vs = Ks + TILE;
-        tile_ready();
-        if (it + 1 < kt.n) {
-            const int j1 = BK * key_tile(kt, it + 1);
-            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
-            sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
-            sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
-        }
-        const int j0 = BK * key_tile(kt, it) + 32 * NS * part;
-        const int kind = tile_kind(p, iw, 32, j0, 32 * NS, len);
-        if (kind) {
+    auto walk = [&](auto fars) {
+        constexpr bool FARS = decltype(fars)::value;
+        for (int it = 0; it < kt.n; ++it) {
+            const T* Ks = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
+            const T* Vs = Ks + TILE;
+            tile_ready();
+            if (it + 1 < kt.n) {
+                const int j1 = BK * key_tile(kt, it + 1);
+                T* nx = lds + ((it + 1) & 1) * 2 * TILE;
+                sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
+                sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
+            }
+            const int j0 = BK * key_tile(kt, it) + 32 * NS * part;
+            const int kind = tile_kind(p, iw, 32, j0, 32 * NS, len);
+            if (kind) {
 #pragma unroll
-            for (int u = 0; u < NS; ++u) {
-                f32x16 s, dp;
+                for (int u = 0; u < NS; ++u) {
+                    f32x16 s, dp;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
+                    for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
 #pragma unroll
-                for (int kk = 0; kk < KD; ++kk) {
-                    Frag<T> a;
-                    row_frag32<DP>(a, Ks, 32 * u, kk, lane);
-                    s = mma32(a, qf[kk], s);
-                    row_frag32<DP>(a, Vs, 32 * u, kk, lane);
-                    dp = mma32(a, df[kk], dp);
-                }
-                if (j0 + 32 * u == iw && __any(rr.lo == ALONE)) {
-                    float own = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) own = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31) ? dp[e] : own;
-                    own = half_sum(own);
-                    if (rr.lo == ALONE && lane < 32) p.delta[((long)b * p.Hq + h) * p.N + i] = own;
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.sc2, -lse)) * (dp[e] - delta);
-                if (kind != ALL) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int j = j0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                        const bool ok = (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
-                        s[e] = ok ? s[e] : 0.f;
-                    }
-                }
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    Frag<T> sf, rest;
-                    acc_frag(sf, s, ks);
-                    if constexpr (FINE) rest_frag(rest, sf, s, ks);
-#pragma unroll
-                    for (int t = 0; t < ND; ++t) {
+                    for (int kk = 0; kk < KD; ++kk) {
                         Frag<T> a;
-                        col_frag32<DP>(a, Ks, 32 * u + 16 * ks, 32 * t, lane);
-                        dq[t] = mma32(a, sf, dq[t]);
-                        if constexpr (FINE) dq[t] = mma32(a, rest, dq[t]);
+                        row_frag32<DP>(a, Ks, 32 * u, kk, lane);
+                        s = mma32(a, qf[kk], s);
+                        row_frag32<DP>(a, Vs, 32 * u, kk, lane);
+                        dp = mma32(a, df[kk], dp);
+                    }
+                    if (j0 + 32 * u == iw && __any(rr.lo == ALONE)) {
+                        float own = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) own = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3) == (lane & 31) ? dp[e] : own;
+                        own = half_sum(own);
+                        if (rr.lo == ALONE && lane < 32) p.delta[((long)b * p.Hq + h) * p.N + i] = own;
+                    }
+                    float ref = lse;
+                    if constexpr (FARS) {
+                        if (far) {
+                            const bool rounded = __any(i < len && beyond(lse, FAR_ROUNDED));
+                            const float inv = 1.f / p.sc2;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const int j = j0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                                const float y = far_exponent(s[e], p.sc2, lse, rounded);
+                                const bool ok = rr.lo == ALONE ? j == i : (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
+                                total += ok ? __builtin_amdgcn_exp2f(y) : 0.f;
+                                s[e] = y * inv;
+                            }
+                            ref = 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.sc2, -ref)) * (dp[e] - delta);
+                    if (kind != ALL) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int j = j0 + 32 * u + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                            const bool ok = (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
+                            s[e] = ok ? s[e] : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        Frag<T> sf, rest;
+                        acc_frag(sf, s, ks);
+                        if constexpr (FINE) rest_frag(rest, sf, s, ks);
+#pragma unroll
+                        for (int t = 0; t < ND; ++t) {
+                            Frag<T> a;
+                            col_frag32<DP>(a, Ks, 32 * u + 16 * ks, 32 * t, lane);
+                            dq[t] = mma32(a, sf, dq[t]);
+                            if constexpr (FINE) dq[t] = mma32(a, rest, dq[t]);
+                        }
                     }
                 }
             }
         }
-    }
+    };
+    if (__builtin_expect(!any_far, 1)) walk(std::false_type{});
+    else walk(std::true_type{});
     __syncthreads();
     if constexpr (KS == 2) {
-        float* x = reinterpret_cast<float*>(smem) + rg * 16 * ND * 64;
-        if (part) half_put(x, dq, lane);
+        float* x = reinterpret_cast<float*>(smem) + rg * (16 * ND + 1) * 64;
+        if (part) {
+            half_put(x, dq, lane);
+            x[16 * ND * 64 + lane] = total;
+        }
         __syncthreads();
-        if (!part) half_add(x, dq, 1.f, 1.f, lane);
+        if (!part) {
+            half_add(x, dq, 1.f, 1.f, lane);
+            total += x[16 * ND * 64 + lane];
+        }
         __syncthreads();
         if (part) return;
     }
-    put_rows<T, DP>(dq, p.scale, i >= len, lds + rg * 32 * C::LD, static_cast<T*>(p.out) + ((long)b * p.N * p.Hq + h) * p.dh,
+    float mul = p.scale;
+    if (far) {
+        total = half_sum(total);
+        if (total == 0.f) total = 1.f;                   // every score is -inf: the row is zero, and stays it
+        mul /= total;
+        if (lane < 32 && i < len) p.shift[((long)b * p.Hq + h) * p.N + i] = -__log2f(total);
+    }
+    put_rows<T, DP>(dq, mul, i >= len, lds + rg * 32 * C::LD, static_cast<T*>(p.out) + ((long)b * p.N * p.Hq + h) * p.dh,
                     (long)p.Hq * p.dh, iw, p.N, p.dh, lane);
 }
 
@@ -767,7 +826,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         if (wave == NW - 1) load_stat<BQ>(p.delta + at, i0, len, ns + BQ, lane);
     };
     // 32 queries of a tile: scores and dP, P and dS from them, then dv and dk
-    auto tile = [&](int kind, const T* Qs, const T* Ds, const float* ls, int u, int i0) {
+    auto tile = [&](auto fars, int kind, const T* Qs, const T* Ds, const float* ls, int u, int i0, int it) {
         f32x16 s, dp;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = dp[e] = 0.f;
@@ -784,11 +843,29 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
                 dp = mma32(a, vf[kk], dp);
             }
         }
+        bool far = false;
+        if constexpr (decltype(fars)::value) {
+            const int r0 = i0 + 32 * u;                  // (before the end, or there would be nothing to see)
+            const long bh = (long)b * p.Hq + hk * p.G + uniform(it / nt);
+            far = uniform(p.far[bh * ((p.N + 31) / 32) + r0 / 32]);
+            if (far) {
+                const float* lse = p.lse + bh * p.N;
+                const bool rounded = __any(beyond(lse[min(r0 + (lane & 31), len - 1)], FAR_ROUNDED));
+                const float inv = 1.f / p.sc2;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int r = min(r0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), len - 1);
+                    asm volatile("" ::: "memory");
+                    s[e] = (far_exponent(s[e], p.sc2, lse[r], rounded) + p.shift[bh * p.N + r]) * inv;
+                }
+            }
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int row = 32 * u + 8 * q + 4 * (lane >> 5);
             asm volatile("" ::: "memory");               // one quarter's statistics in registers at a time
-            const f32x4 L = *reinterpret_cast<const f32x4*>(ls + row), D = *reinterpret_cast<const f32x4*>(ls + BQ + row);
+            f32x4 L = *reinterpret_cast<const f32x4*>(ls + row), D = *reinterpret_cast<const f32x4*>(ls + BQ + row);
+            if (far) L = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float pe = __builtin_amdgcn_exp2f(fmaf(s[4 * q + e], p.sc2, -L[e]));
@@ -826,21 +903,34 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowPa
         }
     };
     if (it0 < it1) fetch(it0);
-    for (int it = it0; it < it1; ++it) {
-        const T* Qs = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
-        const T* Ds = Qs + TILE;
-        const float* ls = stat + (it & 1) * 2 * BQ + 32 * NS * part;
-        tile_ready();
-        if (it + 1 < it1) fetch(it + 1);
-        const int i0 = BQ * (ta + it - uniform(it / nt) * nt) + 32 * NS * part;
-#pragma unroll
-        for (int u = 0; u < NS; ++u) {
-            int kind = jw < len ? tile_kind(p, i0 + 32 * u, 32, jw, 32, len) : 0;
-            // queries past the end: their statistics come as zeros, so p is 1 or more there, and dO's and Q's rows may be others'
-            if (kind && i0 + 32 * u + 32 > len) kind = EDGE_ANY;
-            if (kind) tile(kind, Qs, Ds, ls, u, i0);
+    bool any_far = false;                                // the same for the whole workgroup; read beside the first tile
+    {
+        const int groups = (p.N + 31) / 32, per = BQ / 32;
+        for (int x = it0 * per + lane; x < it1 * per; x += 64) {
+            const int gi = x / (nt * per), at = ta * per + x - gi * (nt * per);
+            any_far |= 32 * at < len && p.far[((long)b * p.Hq + hk * p.G + gi) * groups + at];
         }
+        any_far = __any(any_far);
     }
+    auto walk = [&](auto fars) {
+        for (int it = it0; it < it1; ++it) {
+            const T* Qs = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
+            const T* Ds = Qs + TILE;
+            const float* ls = stat + (it & 1) * 2 * BQ + 32 * NS * part;
+            tile_ready();
+            if (it + 1 < it1) fetch(it + 1);
+            const int i0 = BQ * (ta + it - uniform(it / nt) * nt) + 32 * NS * part;
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+                int kind = jw < len ? tile_kind(p, i0 + 32 * u, 32, jw, 32, len) : 0;
+                // queries past the end: their statistics come as zeros, so p is 1 or more there, and dO's and Q's rows may be others'
+                if (kind && i0 + 32 * u + 32 > len) kind = EDGE_ANY;
+                if (kind) tile(fars, kind, Qs, Ds, ls, u, i0, it);
+            }
+        }
+    };
+    if (any_far) walk(std::true_type{});
+    else walk(std::false_type{});
     if (SINK) {
         float* o = p.part + ((long)id * KS + part) * 2 * DP * 32;
 #pragma unroll
@@ -970,6 +1060,8 @@ Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bo
     }
     return pl;
 }
+// a number for each of N rows or groups in the workspace
+long stat_floats(int B, int Hq, int N) { return ((long)B * Hq * N + 3) / 4 * 4; }
 long part_floats(const Plan& pl, int B, int Hk) { return (long)B * Hk * (pl.sink_keys / 32) * pl.shares * 2 * pl.dp * 32; }
 
 int check_window(const char* what, int dtype, int B, int N, int Hq, int Hk, int dh, float scale, int sinks) {
@@ -1145,7 +1237,7 @@ extern "C" long vitk_window_attn_bwd_workspace_bytes(int dtype, int B, int N, in
     long part = 0;                                       // causal or not, whichever leaves more
     for (int causal = 0; causal < 2; ++causal)
         part = std::max(part, part_floats(make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, causal, true), B, Hk));
-    return ((long)B * Hq * N + 3) / 4 * 16 + part * 4;
+    return (2 * stat_floats(B, Hq, N) + stat_floats(B, Hq, (N + 31) / 32)) * 4 + part * 4;
 }
 
 extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int dh, const void* q, long qb, long qn, long qh,
@@ -1175,7 +1267,9 @@ extern "C" int vitk_window_attn_bwd(int dtype, int B, int N, int Hq, int Hk, int
     p.o_lo = const_cast<void*>(out_lo);
     p.lse = const_cast<float*>(lse);
     p.delta = static_cast<float*>(workspace);
-    p.part = p.delta + ((long)B * Hq * N + 3) / 4 * 4;
+    p.shift = p.delta + stat_floats(B, Hq, N);
+    p.far = reinterpret_cast<int*>(p.shift + stat_floats(B, Hq, N));
+    p.part = p.shift + stat_floats(B, Hq, N) + stat_floats(B, Hq, (N + 31) / 32);
     p.dk = dk;
     p.dv = dv;
     const Plan pl = make_plan(dtype, B, N, Hq, Hk, dh, p.w, p.S, p.causal, p.causal || p.w >= 0 || lengths);
