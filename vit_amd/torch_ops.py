@@ -15,6 +15,7 @@ without any of that state: tensors in, tensors out, compute dtype = the dtype of
     rotary(x[B,N,H,dh], table, pos[B,N]?, offset, interleaved) -> y
     qk_norm_rotary(q, k, gamma_q?, gamma_k?, table?, pos?, offset, eps, interleaved) -> (q', k')
     window_attention(q[B,N,Hq,dh], k, v[B,N,Hk,dh], window, sinks, causal, scale, lengths[B]?) -> (out, lse fp32[B,Hq,N], out_lo)
+        out alone is differentiable
     window_decode(q[B,Hq,dh], k, v[B,Hk,dh], k_cache, v_cache (mutated), lengths, window, sinks, scale) -> out
 
 Reference surfaces: nn.Linear / nn.LayerNorm calls of the encoder layers (model.py:183-204), AttentionLAI.forward
@@ -317,7 +318,7 @@ qk_norm_rotary.register_autograd(_norm_backward, setup_context=_norm_setup)
 @torch.library.custom_op('vit_amd::window_attention', mutates_args=(), device_types='cuda')
 def window_attention(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, causal: bool, scale: float,
                      lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
-    """out_lo: what bf16's rounding took from out, for the backward (empty in fp32)."""
+    """out_lo: what bf16's rounding took from out, for the backward (empty in fp32).  out alone is differentiable."""
     q, k, v = ops._aligned_heads(q), ops._aligned_heads(k), ops._aligned_heads(v)
     out, lse, lo = ops.window_attn_fwd(ops.window_attn_plan(q, k, v, window, sinks, causal, scale, lengths), q, k, v, lengths)
     return out, lse, q.new_empty(0) if lo is None else lo
@@ -346,6 +347,7 @@ def _(dout, q, k, v, out, lse, out_lo, window, sinks, causal, scale, lengths):
 
 def _window_setup(ctx, inputs, output):
     q, k, v, window, sinks, causal, scale, lengths = inputs
+    ctx.mark_non_differentiable(*output[1:])
     ctx.save_for_backward(q, k, v, *output, lengths)
     ctx.cfg = (window, sinks, causal, scale)
 
