@@ -383,8 +383,8 @@ int check_pos(const char* what, const float* table, long rows, int N, int rot, i
     VITK_CHECK_ARG(rot >= 0 && rot % 2 == 0 && rot <= dh, "%s: rotated width %d must be even and at most the head width %d", what, rot, dh);
     if (rot == 0) return VITK_OK;
     VITK_CHECK_ARG(table && (reinterpret_cast<uintptr_t>(table) & 15) == 0, "%s: the table must be 16-byte aligned", what);
-    VITK_CHECK_ARG(ids || (offset >= 0 && offset + N <= rows), "%s: tokens %ld .. %ld are outside the table's %ld rows", what, offset,
-                   offset + N - 1, rows);
+    VITK_CHECK_ARG(ids || (offset >= 0 && offset <= rows - N), "%s: %d tokens from row %ld on are outside the table's %ld rows", what, N,
+                   offset, rows);
     return VITK_OK;
 }
 

@@ -550,6 +550,17 @@ def _aligned_heads(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+# ctypes cuts a number to its C type's bits without a word
+def _i32(n):
+    """An int argument of the C ABI: a count past its range means the same, or is refused the same, as the range's end."""
+    return max(-1, min(int(n), 2 ** 31 - 1))
+
+
+def _sizes(what, *sizes):
+    if max(sizes) > 2 ** 31 - 1:
+        raise ValueError(f'{what}: sizes past 2^31 - 1 are too many for one call, got {sizes}')
+
+
 _POS_KIND = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
 
 
@@ -567,6 +578,7 @@ def rotary_table(positions, freqs, mul=1.0):
         raise ValueError('rotary_table: positions without an axis')
     positions = positions.contiguous()
     P, pairs = positions.shape[0], axes * len(freqs)
+    _sizes('rotary_table', pairs)
     table = torch.empty(P, pairs, 2, device=positions.device, dtype=torch.float32)
     arr = (ctypes.c_double * len(freqs))(*[float(f) for f in freqs])
     check(lib().vitk_rotary_table(_POS_KIND[positions.dtype], axes, P, positions.data_ptr(), pairs,
@@ -585,7 +597,7 @@ def _check_turn(what, B, N, dh, table, pos, offset):
     if 2 * table.shape[1] > dh:
         raise ValueError(f'{what}: the table turns {2 * table.shape[1]} elements of heads of {dh}')
     if pos is None:
-        return int(offset)
+        return max(-1, min(int(offset), 2 ** 62))            # (an end of this range is outside of every table)
     if offset:
         raise ValueError(f'{what}: give pos or offset, not both')
     if tuple(pos.shape) != (B, N) or pos.dtype not in (torch.int32, torch.int64) or not pos.is_contiguous():
@@ -609,6 +621,7 @@ def _turn_args(table, pos, offset):
 def rotary_plan(x, table, pos, offset, interleaved):
     dev = _req_here(x, table, pos)
     (B, N, H, dh), _ = _heads(x, 'rotary x')
+    _sizes('rotary', B, N, H, dh)
     if table is None:
         raise ValueError('rotary: no table')
     return _dt(x), int(interleaved), B, N, H, dh, _check_turn('rotary', B, N, dh, table, pos, offset), dev
@@ -637,6 +650,7 @@ def _check_qk(q, k, gamma_q, gamma_k):
     for g in (gamma_q, gamma_k):
         if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != (dh,) or not g.is_contiguous()):
             raise ValueError('qk_norm_rotary: gamma must be contiguous fp32 [dh]')
+    _sizes('qk_norm_rotary', B, N, Hq, shape[2], dh)
     return B, N, Hq, shape[2], dh, sq, sk
 
 
@@ -692,12 +706,8 @@ def _check_window(q, k, v, window, sinks, lengths):
         raise ValueError('window_attention: sinks must not be negative')
     if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
         raise ValueError('window_attention: lengths must be contiguous int32 [B]')
+    _sizes('window_attention', B, N, Hq)
     return B, N, Hq, Hk, dh, sq, sk, sv
-
-
-def _i32(n):
-    """An int argument of the C ABI: a count past its range means the same as the range's end."""
-    return max(-1, min(int(n), 2 ** 31 - 1))
 
 
 def window_attn_plan(q, k, v, window, sinks, causal, scale, lengths):
@@ -749,6 +759,7 @@ def _check_cache(what, k_cache, v_cache, B, Hk, dh, dtype, lengths):
         raise ValueError(f'{what}: the caches must be contiguous [B, Hk, slots, dh] of the type of k and v')
     if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous()):
         raise ValueError(f'{what}: lengths must be contiguous int32 [B]')
+    _sizes(what, *k_cache.shape)
     return k_cache.shape[2]
 
 
@@ -763,9 +774,10 @@ def window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks, scale):
         raise ValueError('window_decode: lengths are needed')
     B, Hq, dh = q.shape
     Hk = k.shape[1]
+    _sizes('window_decode', Hq)
     C = _check_cache('window_decode', k_cache, v_cache, B, Hk, dh, q.dtype, lengths)
     q, k, v = _aligned_heads(q), _aligned_heads(k), _aligned_heads(v)
-    window, sinks = _i32(window), int(sinks)
+    window, sinks = _i32(window), _i32(sinks)
     L, dt = lib(), _dt(q)
     out = q.new_empty((B, Hq, dh))
     need = L.vitk_window_decode_workspace_bytes(dt, B, Hq, Hk, dh, C, window, sinks)
@@ -783,9 +795,10 @@ def window_cache_fill(k, v, k_cache, v_cache, sinks, lengths=None):
     (B, N, Hk, dh), _ = _heads(k, 'window_cache_fill k')
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError('window_cache_fill: k and v must match')
+    _sizes('window_cache_fill', N)
     C = _check_cache('window_cache_fill', k_cache, v_cache, B, Hk, dh, k.dtype, lengths)
     k, v = _aligned_heads(k), _aligned_heads(v)
     sk, sv = k.stride(), v.stride()
     check(lib().vitk_window_cache_fill(_dt(k), B, N, Hk, dh, k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2],
-                                       _ptr(lengths), k_cache.data_ptr(), v_cache.data_ptr(), C, int(sinks), _stream()),
+                                       _ptr(lengths), k_cache.data_ptr(), v_cache.data_ptr(), C, _i32(sinks), _stream()),
           'vitk_window_cache_fill')
