@@ -95,6 +95,22 @@ template <int DP> __device__ __forceinline__ void row_frag32(Frag<float>& f, con
     }
 }
 
+// part 0: the finite values, 0 for the others; 1: 1 for +inf and NaN, else 0; 2: 1 for -inf and NaN, else 0
+__device__ __forceinline__ void value_part(Frag<float>& f, int part) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float x = f.v[e];
+        const bool finite = fabsf(x) < INFINITY;
+        f.v[e] = part == 0 ? (finite ? x : 0.f) : (finite || x == (part == 1 ? -INFINITY : INFINITY) ? 0.f : 1.f);
+    }
+}
+__device__ __forceinline__ void value_part(Frag<__bf16>& f, int part) {
+    const s16x8 x = __builtin_bit_cast(s16x8, f.v), beyond = (x & (short)0x7f80) == (short)0x7f80;      // all bits where not finite
+    s16x8 y = x & ~beyond;
+    if (part) y = beyond & (x != (short)(part == 1 ? 0xff80 : 0x7f80)) & (short)0x3f80;
+    f.v = __builtin_bit_cast(bf16x8, y);
+}
+
 struct View {                     // element (b, n, h, d) at b*sb + n*sn + h*sh + d
     const void* p;
     long sb, sn, sh;
@@ -366,110 +382,184 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
     const KeyTiles kt = key_tiles(p, i0, i0 + 32 * RG, len, BK);
     const RowRange rr = row_range(p, i, len);
     f32x16 o[ND];
-#pragma unroll
-    for (int t = 0; t < ND; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
-    float m = -INFINITY;                                 // running maximum, log2 domain
-    float ls[4] = {0.f, 0.f, 0.f, 0.f};                  // the sum of this lane's keys, in four chains
+    float m;                                             // running maximum, log2 domain
+    float ls[4];                                         // the sum of this lane's keys, in four chains
 
     loads_done();                                        // nothing but tiles is in flight in the loop
     Stager<T, DP, BK, NT> sk, sv;
     sk.init(p.k.sn, p.dh);
     sv.init(p.v.sn, p.dh);
-    if (kt.n > 0) {
-        const int j0 = BK * key_tile(kt, 0);
-        sk.load(K, p.k.sn, j0, len, p.dh, lds, wave);
-        sv.load(V, p.v.sn, j0, len, p.dh, lds + TILE, wave);
-    }
-    for (int it = 0; it < kt.n; ++it) {
-        const T* Ks = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
-        const T* Vs = Ks + TILE;
-        tile_ready();                                    // and the other buffer's readers are done
-        if (it + 1 < kt.n) {
-            const int j1 = BK * key_tile(kt, it + 1);
-            T* nx = lds + ((it + 1) & 1) * 2 * TILE;
-            sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
-            sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
+    auto walk = [&](auto careful) {
+        m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ls[e] = 0.f;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
+        if (kt.n > 0) {
+            const int j0 = BK * key_tile(kt, 0);
+            sk.load(K, p.k.sn, j0, len, p.dh, lds, wave);
+            sv.load(V, p.v.sn, j0, len, p.dh, lds + TILE, wave);
         }
-        const int j0 = BK * key_tile(kt, it) + 32 * NS * part;
-        const int kind = tile_kind(p, iw, 32, j0, 32 * NS, len);         // the same for the whole wave
-        if (kind) {
-            f32x16 s[NS];
-            float mt = -INFINITY;
+        for (int it = 0; it < kt.n; ++it) {
+            const T* Ks = lds + (it & 1) * 2 * TILE + part * (32 * NS * DP);
+            const T* Vs = Ks + TILE;
+            tile_ready();                                    // and the other buffer's readers are done
+            if (it + 1 < kt.n) {
+                const int j1 = BK * key_tile(kt, it + 1);
+                T* nx = lds + ((it + 1) & 1) * 2 * TILE;
+                sk.load(K, p.k.sn, j1, len, p.dh, nx, wave);
+                sv.load(V, p.v.sn, j1, len, p.dh, nx + TILE, wave);
+            }
+            const int j0 = BK * key_tile(kt, it) + 32 * NS * part;
+            const int kind = tile_kind(p, iw, 32, j0, 32 * NS, len);         // the same for the whole wave
+            if (kind) {
+                f32x16 s[NS];
+                float mt = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < NS; ++u) {
+                for (int u = 0; u < NS; ++u) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
+                    for (int e = 0; e < 16; ++e) s[u][e] = 0.f;
 #pragma unroll
-                for (int kk = 0; kk < KD; ++kk) {
-                    Frag<T> a;
-                    row_frag32<DP>(a, Ks, 32 * u, kk, lane);
-                    s[u] = mma32(a, qf[kk], s[u]);
+                    for (int kk = 0; kk < KD; ++kk) {
+                        Frag<T> a;
+                        row_frag32<DP>(a, Ks, 32 * u, kk, lane);
+                        s[u] = mma32(a, qf[kk], s[u]);
+                    }
                 }
-            }
-            if (kind != ALL) hide(s, kind, rr, j0, lane);
+                if (kind != ALL) hide(s, kind, rr, j0, lane);
 #pragma unroll
-            for (int u = 0; u < NS; ++u)
+                for (int u = 0; u < NS; ++u)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
-            mt = half_max(mt) * p.sc2;
-            // the reference point only has to keep exp2 in range: it moves when a row's maximum has grown by 2^8
-            if (__any(mt > m + 8.f)) {
-                const float mn = fmaxf(m, mt);
-                const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
+                    for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
+                mt = half_max(mt) * p.sc2;
+                // the reference point only has to keep exp2 in range: it moves when a row's maximum has grown by 2^8
+                if (__any(mt > m + 8.f)) {
+                    const float mn = fmaxf(m, mt);
+                    const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ls[e] *= al;
+                    for (int e = 0; e < 4; ++e) ls[e] *= al;
 #pragma unroll
-                for (int t = 0; t < ND; ++t)
+                    for (int t = 0; t < ND; ++t)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[t][e] *= al;
-            }
-            const float mr = m == -INFINITY ? 0.f : m;
-            if (__any(fabsf(mr) > 16777216.f)) {         // out here the product's rounding, which m has and the fma has not,
+                        for (int e = 0; e < 16; ++e) o[t][e] *= al;
+                }
+                const float mr = m == -INFINITY ? 0.f : m;
+                if (__any(fabsf(mr) > 16777216.f)) {         // out here the product's rounding, which m has and the fma has not,
 #pragma unroll                                           // would be an exponent of its own
+                    for (int u = 0; u < NS; ++u)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float x = s[u][e] * p.sc2;
+                            asm("" : "+v"(x));               // two roundings: not to be contracted
+                            s[u][e] = x - mr;
+                        }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < NS; ++u)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[u][e] = fmaf(s[u][e], p.sc2, -mr);
+                }
+                if constexpr (decltype(careful)::value) {                // no visible key's p is 0
+#pragma unroll
+                    for (int u = 0; u < NS; ++u)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[u][e] = s[u][e] < -120.f && s[u][e] > -INFINITY ? -120.f : s[u][e];
+                }
+#pragma unroll
                 for (int u = 0; u < NS; ++u)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        float x = s[u][e] * p.sc2;
-                        asm("" : "+v"(x));               // two roundings: not to be contracted
-                        s[u][e] = x - mr;
+                        s[u][e] = __builtin_amdgcn_exp2f(s[u][e]);
+                        ls[e & 3] += s[u][e];
                     }
-            } else {
+                if constexpr (decltype(careful)::value) {
+#pragma unroll
+                    for (int t = 0; t < ND; ++t) {
+#pragma unroll
+                        for (int part = 0; part < 3; ++part) {           // the finite values, then where +inf and -inf go
+                            f32x16 c = o[t];
+                            if (part) {
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) c[e] = 0.f;
+                            }
+#pragma unroll
+                            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                                for (int ks = 0; ks < 2; ++ks) {
+                                    Frag<T> a, pf, rest;
+                                    asm volatile("" ::: "memory");       // one product's operands in registers at a time
+                                    __builtin_amdgcn_sched_barrier(0);
+                                    int l2 = lane;
+                                    asm volatile("" : "+v"(l2));
+                                    col_frag32<DP>(a, Vs, 32 * u + 16 * ks, 32 * t, l2);
+                                    value_part(a, part);
+                                    acc_frag(pf, s[u], ks);
+                                    if constexpr (FINE) {
+                                        rest_frag(rest, pf, s[u], ks);
+                                        if (!part) c = mma32(a, rest, c);
+                                    }
+                                    if (part) {
+#pragma unroll
+                                        for (int e = 0; e < 8; ++e) frag_set_f(pf, e, s[u][8 * ks + e] > 0.f ? 1.f : 0.f);
+                                    }
+                                    c = mma32(a, pf, c);
+                                }
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                if (!part) o[t][e] = c[e];
+                                else o[t][e] += c[e] > 0.f ? (part == 1 ? INFINITY : -INFINITY) : 0.f;
+                            }
+                        }
+                    }
+                } else
 #pragma unroll
                 for (int u = 0; u < NS; ++u)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s[u][e] = fmaf(s[u][e], p.sc2, -mr);
-            }
+                    for (int ks = 0; ks < 2; ++ks) {
+                        Frag<T> pf, rest;
+                        acc_frag(pf, s[u], ks);
+                        if constexpr (FINE) rest_frag(rest, pf, s[u], ks);
 #pragma unroll
-            for (int u = 0; u < NS; ++u)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[u][e] = __builtin_amdgcn_exp2f(s[u][e]);
-                    ls[e & 3] += s[u][e];
-                }
-#pragma unroll
-            for (int u = 0; u < NS; ++u)
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    Frag<T> pf, rest;
-                    acc_frag(pf, s[u], ks);
-                    if constexpr (FINE) rest_frag(rest, pf, s[u], ks);
-#pragma unroll
-                    for (int t = 0; t < ND; ++t) {
-                        Frag<T> a;
-                        col_frag32<DP>(a, Vs, 32 * u + 16 * ks, 32 * t, lane);
-                        o[t] = mma32(a, pf, o[t]);
-                        if constexpr (FINE) o[t] = mma32(a, rest, o[t]);
+                        for (int t = 0; t < ND; ++t) {
+                            Frag<T> a;
+                            col_frag32<DP>(a, Vs, 32 * u + 16 * ks, 32 * t, lane);
+                            o[t] = mma32(a, pf, o[t]);
+                            if constexpr (FINE) o[t] = mma32(a, rest, o[t]);
+                        }
                     }
-                }
+            }
         }
-    }
+    };
+    walk(std::false_type{});
     float l = half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
+    // A non-finite V of a key that only some queries of a tile see has reached the others as 0 * V.  Where a result is not finite,
+    // the workgroup walks again and multiplies the finite values, and 0 and 1 for the infinities, apart.  (FINE: p and its
+    // remainder can be of two signs, and infinity times both is no number.  V rows that share memory: what lies behind the last
+    // one is hidden too.)
+    __shared__ int again[NW];
+    {
+        float bad = 0.f;
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) bad += o[t][e] * 0.f;
+        const bool redo = __any(i < len && bad != 0.f && l == l);        // (a NaN is unequal; a NaN sum is the row's own)
+        if (lane == 0) again[wave] = redo;
+    }
+    __syncthreads();                                     // everyone is done with the tiles
+    int redo = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) redo |= again[w];
+    if (__builtin_expect((FINE || p.w >= 0 || p.causal || p.v.sn < p.dh) && uniform(redo), 0)) {
+        walk(std::true_type{});
+        l = half_sum((ls[0] + ls[1]) + (ls[2] + ls[3]));
+        __syncthreads();
+    }
     if constexpr (KS == 2) {
         float* x = reinterpret_cast<float*>(smem) + rg * (16 * ND + 2) * 64;
-        __syncthreads();
         if (part) {
             half_put(x, o, lane);
             x[16 * ND * 64 + lane] = m;
@@ -487,53 +577,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowPa
         if (part) return;
     }
     const bool none = i >= len || (m == -INFINITY && l == 0.f);      // nothing visible (a NaN sum stays a NaN)
-    // A non-finite V of a key that only some queries of a tile see has reached the others as 0 * V.  Where the result is not
-    // finite, it is made again key by key, for the keys that each query sees.  (FINE: p and its remainder can be of two signs,
-    // and infinity times both is no number.  V rows that share memory: so has what lies behind the last one.)
-    float bad = 0.f;
-#pragma unroll
-    for (int t = 0; t < ND; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) bad += o[t][e] * 0.f;
-    if ((FINE || p.w >= 0 || p.causal || p.v.sn < p.dh) && __any(!none && bad != 0.f && l == l)) {         // (a NaN is unequal; a NaN sum is the row's own)
-#pragma unroll
-        for (int t = 0; t < ND; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[t][e] = 0.f;
-        const int first = p.w < 0 ? 0 : max(0, iw - p.w), last = min(len, p.causal ? iw + 32 : (p.w < 0 ? len : iw + 32 + p.w));
-        const int sinks = min(p.S, len);
-        const float mr = m == -INFINITY ? 0.f : m;
-        for (int x = 0; x < sinks + max(0, last - first); ++x) {
-            const int j = x < sinks ? x : first + x - sinks;
-            if (x >= sinks && j < sinks) continue;       // a sink: had its turn
-            float s = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < KD; ++kk) {
-                const int d = 16 * kk + 8 * (lane >> 5);
-                if (d < p.dh) {
-                    Frag<T> a;
-                    frag_load(a, K + (long)j * p.k.sn + d);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s += frag_get_f(a, e) * frag_get_f(qf[kk], e);
-                }
-            }
-            s = half_sum(s) * p.sc2;
-            const bool ok = (unsigned)(j - rr.lo) <= rr.span || j < rr.s;
-            const float pj = __builtin_amdgcn_exp2f(s - mr);
-#pragma unroll
-            for (int t = 0; t < ND; ++t)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int d = 32 * t + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                    if (d < p.dh) {
-                        const float y = o[t][e] + pj * to_f32(V[(long)j * p.v.sn + d]);
-                        o[t][e] = ok ? y : o[t][e];
-                    }
-                }
-        }
-    }
     if (p.lse && lane < 32 && i < p.N) p.lse[((long)b * p.Hq + h) * p.N + i] = none ? INFINITY : m + __log2f(l);
-    if constexpr (KS == 1) __syncthreads();
     const long at = ((long)b * p.N * p.Hq + h) * p.dh, ldg = (long)p.Hq * p.dh;
     T* mine = lds + rg * 32 * C::LD;
     put_rows<T, DP>(o, 1.f / l, none, mine, static_cast<T*>(p.out) + at, ldg, iw, p.N, p.dh, lane);
