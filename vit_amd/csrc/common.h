@@ -133,14 +133,15 @@ __device__ __forceinline__ float gelu_grad_fast(float x) {
     return fmaf(0.5f, erfv, 0.5f) + x * (0.39894228040143267794f * e);
 }
 
-// erf-GELU without transcendentals, two elements per instruction (v_pk_fma_f32): round 3's form of the bf16 epilogues.
+// erf-GELU without transcendentals, two elements side by side: the form of the bf16 epilogues.
 //   gelu(x)  = x / 2 + E(x),   E(x) = x (Phi(x) - 1/2)   even, = x^2 P(z) on |x| <= 4,  z = x^2 / 8 - 1 in [-1, 1]
 //   gelu'(x) = 1 / 2 + x R(z)                                                                (R fitted on its own)
 // P, R: degree-8 least-squares fits on Chebyshev nodes (tools/fit_gelu.py), evaluated by Horner in z; |x| > 4 continues the
 // value at 4 with slope 1 / 0 (gelu) or holds it (gelu').  Max |error| in fp32 Horner: 9.5e-5 (gelu, in the tails; 3e-5
 // inside), 6e-4 (gelu', tails; 1.1e-4 inside) -- an order below the 2^-9 rounding of the bf16 value it is stored as, and
-// 10.5 VALU per element where the exp2 / rcp form above costs 12 + two quarter-rate ops: the fc1 forward and fc2 dX GEMMs
-// spent a fifth of their time in this arithmetic with the matrix cores idle.
+// 16 (gelu) and 12 (gelu') VALU per element where the exp2 / rcp form above costs 13 and 14 with two quarter-rate ops more (the
+// library is built without packed fp32 instructions, which would take two elements each): the fc1 forward and fc2 dX GEMMs
+// spent a fifth of their time in the older form with the matrix cores idle.
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 __device__ __forceinline__ f32x2 gelu_clamp2(f32x2 x) {
     return f32x2{__builtin_amdgcn_fmed3f(x[0], -4.f, 4.f), __builtin_amdgcn_fmed3f(x[1], -4.f, 4.f)};

@@ -352,9 +352,10 @@ template <int ND> __device__ __forceinline__ void half_add(const float* x, f32x1
 // Tiles come by asynchronous loads into one of two images while the other is used, one barrier a tile.  Bound by the matrix
 // unit and the softmax's vector work in turn (32 exponentials, maxima, sums and conversions of them beside 32 MFMA a wave and
 // tile of 64 keys of 128): two waves a SIMD cover each other's, and no part taken out by itself gives more than 15 %.
-// bf16, heads of 128: 8192 tokens x 16 heads, causal, 290 us = 950 TFLOP/s of visible pairs; 16384 tokens with a causal window
-// of 1024 181 us = 740, a ninth of whose pairs are the window's and the diagonal's edges and are thrown away.  fp32, heads of 80:
-// 4 x 1001 x 16 196 us = 105 TFLOP/s of 154.
+// bf16, heads of 128: 8192 tokens x 16 heads, causal, 287 us = 960 TFLOP/s of visible pairs; 16384 tokens with a causal window
+// of 1024 174 to 187 us by machine = 720 to 770, a ninth of whose pairs are the window's and the diagonal's edges and are thrown
+// away (launches one after another; a profiler, which parts them, has 200 to 215).  fp32: 4 x 1001 x 16 heads of 80 195 us = 105
+// TFLOP/s of 154; 2 x 2048 x 16 of 128, causal, 357 us = 96.
 template <typename T, int HW, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_fwd_kernel(const WindowParams p) {
     constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
@@ -598,7 +599,7 @@ __device__ __forceinline__ float far_exponent(float s, float sc2, float lse, boo
 }
 
 // ------------------------------------------------------------------------------------- backward: dq (and D for the other)
-// The forward's walk with three products (S, dP, dS K); 270 us = 740 TFLOP/s at the forward's windowed size.
+// The forward's walk with three products (S, dP, dS K); 275 us = 730 TFLOP/s at the forward's windowed size.
 template <typename T, int HW, int NW, int KS, int BK, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowParams p) {
     constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
@@ -781,7 +782,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void window_dq_kernel(const WindowPar
 // A wave owns 32 keys (a lane one key, scores S[query][key]); the workgroup walks the query tiles that can see its keys, for
 // every head of the group.  KS waves share 32 keys, each with its own part of every query tile.  SINK: the 32 keys of a sinks'
 // tile and a share of ALL the query tiles, each wave's sums out in fp32 (window_sink_sum_kernel adds the shares in order).
-// Four products (S, dP, P dO, dS Q) on the same two operands: 300 us = 890 TFLOP/s at the forward's windowed size.
+// Four products (S, dP, P dO, dS Q) on the same two operands: 320 us = 830 TFLOP/s at the forward's windowed size.  fp32 is one
+// wave a SIMD from 80 wide heads on (194 + 128 registers): 4 x 1001 x 16 of 80 672 us for the whole backward.
 template <typename T, int HW, int NW, int KS, int BQ, bool SINK, bool VLDS, int WPE, bool FINE>
 __global__ __launch_bounds__(64 * NW, WPE) void window_dkv_kernel(const WindowParams p) {
     constexpr int DP = (HW + 31) / 32 * 32;              // the width of the images
@@ -1058,28 +1060,28 @@ constexpr int NARROW = 256;
 
 // Up to how many workgroups of 128 rows there are, that workgroups of 64 with two waves a row, each with half of the other axis,
 // are faster.  One of 128 takes as long as its longest row, whatever the other CUs do: few of them leave CUs, and a second
-// round of them most of its CUs, waiting.  Halves read every tile for half the rows.  fp32, 16 heads x 1001 tokens of 80 (as 96), forward
-// and backward: one sequence 68 + 205 us against 120 + 390, three 200 + 608 against 209 + 749, four 265 + 808 against 211 +
-// 759; causal, four of 1024: 201 + 605 against 210 + 746.  bf16, 16 x 1024: heads of 128 24 + 59 against 31 + 93, two sequences
-// 31 + 99 against 34 + 95, three 47 + 149 against 41 + 118; of 64 three 26 + 75 against 28 + 76, four 33 + 92 against 30 + 83.
+// round of them most of its CUs, waiting.  Halves read every tile for half the rows.  fp32, 16 heads x 1001 tokens of 80, forward
+// and backward: one sequence 67 + 192 us against 113 + 349, three 186 + 571 against 193 + 664, four 249 + 763 against 195 +
+// 673; causal, four of 1024: 143 + 436 against 148 + 436.  bf16, 16 x 1024: heads of 128, causal, 23 + 62 against 30 + 95, two
+// sequences 26 + 74 against 32 + 96, three 34 + 108 against 33 + 102; of 64 three 26 + 75 against 27 + 79, four 32 + 94 against 29 + 83.
 long halves_up_to(int dtype, int dp, bool uneven) { return dtype == VITK_F32 ? (uneven ? 512 : 384) : (dp <= 64 ? 384 : 256); }
 
 Plan make_plan(int dtype, int B, int N, int Hq, int Hk, int dh, int w, int S, bool causal, bool uneven) {
     Plan pl;
     pl.dp = (dh + 31) / 32 * 32;
-    pl.width = dh > 64 && dh <= 80 ? 80 : pl.dp;         // (4 x 1001 x 16 heads of 80, fp32: 196 + 696 us
-                                                         // forward and backward; as 96, a sixth more steps, 210 + 755; bf16 40 + 110, 41 + 114)
+    pl.width = dh > 64 && dh <= 80 ? 80 : pl.dp;         // (4 x 1001 x 16 heads of 80, fp32: 195 + 672 us
+                                                         // forward and backward; as 96, a sixth more steps, 209 + 730; bf16 40 + 114, 39 + 120)
     // P and dS are rounded to bf16 for their products, an error of the size of the results' own rounding as long as many share in
     // it.  In a call of few scores single ones can carry dq and dk (up to 87 tokens, window 2: 0.0021 of the norm before the
     // result's own rounding, 0.0017 in large calls): there what the rounding took is multiplied too, in the forward as well,
-    // whose error dq and dk have through o . do (256 tokens x 4 heads of 64: forward 9.4 us against 8.6, backward 23.9 against
-    // 21.5).
+    // whose error dq and dk have through o . do (180 tokens x 4 heads of 64: forward 8.1 us against 7.7, backward 18.6 against
+    // 17.4).
     const long keys = w < 0 ? N : (2L * w + 1 + S < N ? 2L * w + 1 + S : N);
     pl.fine = dtype == VITK_BF16 && (long)B * Hq * N * keys <= FINE;
     const long tq = (long)B * Hq * ((N + 127) / 128), tk = (long)B * Hk * ((N + 127) / 128), most = halves_up_to(dtype, pl.dp, uneven);
     pl.halves_q = pl.fine || tq <= most;
     // (causal without a window: the first keys' rows are twice the average, times the group's heads.  8 ragged sequences up to 1500
-    // x 16 heads of 80 in groups of 4: the backward 202 us against 303; 2 x 8192 x 12 of 64 in groups of 3: 879 against 996)
+    // x 16 heads of 80 in groups of 4: the backward 198 us against 283; 2 x 8192 x 12 of 64 in groups of 3: 866 against 1013)
     pl.halves_k = pl.fine || tk <= (dtype == VITK_BF16 && causal && w < 0 ? 2 * most : most);
     // The sinks' keys are seen by all N queries, the 128 of another tile by `near` of them.  Where that is over four times more, or
     // so much that the ordinary launch would wait for the sinks' tiles, they get a launch of their own, whose workgroups share
@@ -1137,11 +1139,11 @@ void fill_params(WindowParams& p, int B, int N, int Hq, int Hk, int dh, int w, i
 }
 // Sets the order of the (tile, sequence, key head) pieces of `each` neighbours, and the grid that goes with it.  By tile, the long
 // ones first, dealt to the XCDs in turn: where pieces differ (sequences of different lengths, causal rows without a window:
-// 8192 tokens x 16 heads of 128, groups of 4, forward and backward 290 + 1214 us; in runs of 16 to each XCD, some of which then
-// had all the long ones, 405 + 2147), and where heads are a multiple of 8, so that a head stays on one XCD (16 x 577 x 12 heads
-// of 64, window 64: 20 + 62 us against 22 + 66).  A multiple of 8 heads whose tiles differ by the sequence alone: whole heads to
-// each XCD in turn (1001, 100 and 1001 tokens x 16 heads of 80, fp32: 138 + 411 us against 188 + 559 by tile).  Else an eighth of
-// the pieces in a row to each XCD (16384 tokens, groups of 4 heads of 128, window 1024: 181 + 555 us against 183 + 567).
+// 8192 tokens x 16 heads of 128, groups of 4, forward and backward 298 + 1265 us; an eighth of them in a row to each XCD, some of
+// which then had all the long ones, 395 + 1795), and where heads are a multiple of 8, so that a head stays on one XCD (16 x 577 x
+// 12 heads of 64, window 64: 21 + 65 us against 23 + 74).  A multiple of 8 heads whose tiles differ by the sequence alone: whole
+// heads to each XCD in turn (1001, 100 and 1001 tokens x 16 heads of 80, fp32: 137 + 418 us against 186 + 570 by tile).  Else an
+// eighth of the pieces in a row to each XCD (16384 tokens, groups of 4 heads of 128, window 1024: 180 + 576 us against 185 + 586).
 unsigned xcd_grid(WindowParams& p, int tiles, int each, bool by_tile) {
     const int heads = p.B * p.Hk, total = heads * tiles * each;
     p.total = total;
@@ -1172,8 +1174,8 @@ template <typename T, int HW, int KS, int BK, bool FINE = false> void run_fwd_ti
     hipLaunchKernelGGL((window_fwd_kernel<T, HW, NW, KS, BK, WPE, FINE>), dim3(grid), dim3(64 * NW), lds, st, p);
 }
 // Key tiles of 64 in bf16; of 32 where the window is narrow and a tile of 64 would be mostly edge (16 x 577 tokens x 12 heads of
-// 64, window 64 on both sides: 24.1 us against 27.1, window 256: 33.5 against 34.7; 2 x 8192 x 16 heads of 128, causal window
-// of 512: 124.4 against 123.0, 16384 x 16, of 1024: 222 against 190).
+// 64, window 64 on both sides: 22.9 us against 25.6, window 256: 30.7 against 31.4; 2 x 8192 x 16 heads of 128, causal window
+// of 512: 131 against 126, 16384 x 16, of 1024: 200 against 186).
 template <typename T, int HW> void run_fwd(const WindowParams& p, const Plan& pl, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
         if (pl.fine) return run_fwd_tiles<T, HW, 2, 64, true>(p, st);

@@ -260,7 +260,8 @@ __global__ __launch_bounds__(64 * NW) void window_decode_kernel(const DecodePara
 // keys 4 (l >> 4) .. + 3 in its registers; V is read so that the same 16 lanes hold those 4 keys' rows, and a probability
 // reaches the row's lanes by a broadcast within 16 lanes.  On the vector unit the scores took 8 products, 8 conversions and
 // 4 exchanges a head and 16 bytes of K: 64 sequences x 4 key heads x 4 x 4100 keys of 128 (447 MB, the caches
-// part full) took 222 us in place of 87 (5.1 TB/s, a large copy's rate).
+// part full) took 222 us in place of 87 (5.1 TB/s, a large copy's rate).  (fp32 takes the vector unit's kernel: full caches of
+// that size, 1075 MB, 194 us = 5.5 TB/s, so its bytes bound it there too; bf16 101 us = 5.3.)
 typedef __attribute__((ext_vector_type(4))) float f32v4;
 template <int LPK, int GB, int NW>
 __global__ __launch_bounds__(64 * NW) void window_decode_group_kernel(const DecodeParams p) {

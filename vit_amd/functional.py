@@ -1182,8 +1182,10 @@ def window_attention(q, k, v, window, sinks=0, causal=False, scale=None, lengths
     query i sees the keys j with |i - j| <= window, and the first ``sinks`` keys (class / register tokens) wherever it is;
     ``causal``: of those only j <= i.  window < 0: every key.  ``lengths`` (int32 [B]): tokens of each padded sequence; rows past
     it are not read, and their outputs and gradients are 0.  scale: dh^-0.5 unless given (positive).  out [B, N, Hq, dh],
-    contiguous.  Non-finite values reach the outputs of the rows that see them and no others; in the backward also the gradients
-    of rows and keys around them."""
+    contiguous; a row whose every score is -inf is 0.  Non-finite values reach the outputs of the rows that see them and no others
+    (such a call takes up to 7 times as long); in the backward also the gradients of rows and keys around them.  bf16: P and dS are rounded
+    to bf16 for their products where a call has more than 2^17 scores (B * Hq * N * visible keys), so a sequence's last bits can
+    differ with the batch that it is in."""
     return WindowAttentionFn.apply(q, k, v, window, sinks, causal, q.shape[-1] ** -0.5 if scale is None else scale, lengths)
 
 
