@@ -1203,7 +1203,7 @@ def window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks=0, scale=Non
 
 
 def window_cache_fill(k, v, k_cache, v_cache, sinks=0, lengths=None):
-    """The k and v [B, N, Hk, dh] of whole prompts (``lengths``: int32 [B] of padded ones) into the empty ring caches of
+    """The k and v [B, N, Hk, dh] (any strides) of whole prompts (``lengths``: int32 [B] of padded ones) into the empty ring caches of
     ``window_decode``, in place: every slot takes the last token that belongs in it, the others are left as they are.  No backward."""
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise RuntimeError('window_cache_fill has no backward: call it under torch.no_grad()')

@@ -792,12 +792,12 @@ def window_decode(q, k, v, k_cache, v_cache, lengths, window, sinks, scale):
 def window_cache_fill(k, v, k_cache, v_cache, sinks, lengths=None):
     """The prompts' k / v [B, N, Hk, dh] into empty ring caches, in place."""
     _req_here(k, v, k_cache, v_cache, lengths)
+    k, v = _aligned_heads(k), _aligned_heads(v)
     (B, N, Hk, dh), _ = _heads(k, 'window_cache_fill k')
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError('window_cache_fill: k and v must match')
     _sizes('window_cache_fill', N)
     C = _check_cache('window_cache_fill', k_cache, v_cache, B, Hk, dh, k.dtype, lengths)
-    k, v = _aligned_heads(k), _aligned_heads(v)
     sk, sv = k.stride(), v.stride()
     check(lib().vitk_window_cache_fill(_dt(k), B, N, Hk, dh, k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2],
                                        _ptr(lengths), k_cache.data_ptr(), v_cache.data_ptr(), C, _i32(sinks), _stream()),
